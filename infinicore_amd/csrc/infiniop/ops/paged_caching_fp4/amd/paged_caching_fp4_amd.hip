@@ -1,0 +1,245 @@
+// paged_caching_fp4 on AMD Instinct (gfx950): quantise the K and V vectors of a chunk of tokens and scatter them into their
+// slots of a pool held in 4 bits.
+//
+// Per 32 elements x: s = clamp(floor(log2 max|x|) - 2, -23, 13), code = e2m1 nearest to x 2^-s, held at 6. A lane takes eight
+// elements (one 16-byte load of 16-bit values), so a group is four lanes: the largest magnitude passes between them in two
+// data-parallel moves, the conversion instruction takes pairs with the scale, and a lane leaves one dword of codes, the
+// first of the four also the scale byte. Scales are powers of two, so the quotient is exact and a code has one right value.
+// K and V of a token follow one another in the numbering of the lanes: eight KV heads of 128 are one workgroup per token.
+#include "paged_caching_fp4_amd.h"
+#include "../../../devices/amd/amd_fp4.h"
+#include "../../../devices/amd/amd_streaming.h"
+#include "../../../handle.h"
+#include "../../../../utils/check.h"
+
+namespace op::paged_caching_fp4::amd {
+
+namespace {
+
+using namespace device::amd;
+
+constexpr int kThreads = 256;
+constexpr int kPerLane = 8; // elements
+
+struct Side { // keys or values
+    uint8_t *codes, *scales;
+    const void *source;
+    int64_t code_block, code_head, code_row;    // bytes
+    int64_t scale_block, scale_head, scale_row; // bytes
+    int64_t token_stride, head_stride;          // elements
+    uint32_t lanes_per_row;                     // size / 8
+};
+
+struct QuantArgs {
+    Side k, v;
+    const int64_t *slot_mapping;
+    int64_t num_slots;
+    uint32_t num_tokens;
+    uint32_t k_lanes;     // of a token: heads x k.lanes_per_row
+    uint32_t token_lanes; // of its keys and values
+    uint32_t block_tokens; // tokens of a workgroup
+    uint32_t block_size;
+    int32_t block_shift;  // log2(block_size) when it is a power of two, else -1
+};
+
+// Largest magnitude among the four lanes of a group, by the bits: of non-negative floats they are ordered as the values are,
+// and a NaN stays above infinity.
+__device__ __forceinline__ uint32_t groupMax(uint32_t x) {
+    x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0xB1, 0xf, 0xf, true))); // lanes 1 0 3 2
+    x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), 0x4E, 0xf, 0xf, true))); // lanes 2 3 0 1
+    return x;
+}
+
+// Eight elements as loaded, their largest magnitude (bits of a float) and their codes.
+struct EightBF16 {
+    using Element = uint16_t;
+    uint4 w;
+    __device__ __forceinline__ uint32_t top() const {
+        const uint32_t m = 0x7fff7fffu;
+        const uint32_t a = max16(max16(w.x & m, w.y & m), max16(w.z & m, w.w & m));
+        const uint32_t hi = a >> 16, lo = a & 0xffffu;
+        return (hi > lo ? hi : lo) << 16;
+    }
+    __device__ __forceinline__ uint32_t codes(float s) const {
+        return mx::fromBF16<3>(mx::fromBF16<2>(mx::fromBF16<1>(mx::fromBF16<0>(0, w.x, s), w.y, s), w.z, s), w.w, s);
+    }
+    static __device__ __forceinline__ uint32_t max16(uint32_t a, uint32_t b) {
+        typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+    }
+    __device__ __forceinline__ void load(const Element *p) { w = loadStreamed<uint4>(p); }
+    __device__ __forceinline__ void loadEach(const Element *p) {
+        w = make_uint4(p[0] | p[1] << 16, p[2] | p[3] << 16, p[4] | p[5] << 16, p[6] | p[7] << 16);
+    }
+};
+struct EightF16 : EightBF16 {
+    __device__ __forceinline__ uint32_t top() const {
+        const uint32_t m = 0x7fff7fffu;
+        const uint32_t a = max16(max16(w.x & m, w.y & m), max16(w.z & m, w.w & m));
+        const uint32_t hi = a >> 16, lo = a & 0xffffu;
+        const uint16_t t = static_cast<uint16_t>(hi > lo ? hi : lo);
+        return __float_as_uint(static_cast<float>(__builtin_bit_cast(_Float16, t)));
+    }
+    __device__ __forceinline__ uint32_t codes(float s) const {
+        return mx::fromF16<3>(mx::fromF16<2>(mx::fromF16<1>(mx::fromF16<0>(0, w.x, s), w.y, s), w.z, s), w.w, s);
+    }
+};
+struct EightF32 {
+    using Element = float;
+    uint4 a, b;
+    __device__ __forceinline__ uint32_t top() const {
+        const uint32_t m = 0x7fffffffu;
+        return max(max(max(a.x & m, a.y & m), max(a.z & m, a.w & m)), max(max(b.x & m, b.y & m), max(b.z & m, b.w & m)));
+    }
+    __device__ __forceinline__ uint32_t codes(float s) const {
+        auto f = [](uint32_t x) { return __uint_as_float(x); };
+        return mx::fromF32<3>(mx::fromF32<2>(mx::fromF32<1>(mx::fromF32<0>(0, f(a.x), f(a.y), s), f(a.z), f(a.w), s),
+                                               f(b.x), f(b.y), s), f(b.z), f(b.w), s);
+    }
+    __device__ __forceinline__ void load(const Element *p) {
+        a = loadStreamed<uint4>(p);
+        b = loadStreamed<uint4>(p + 4);
+    }
+    __device__ __forceinline__ void loadEach(const Element *p) {
+        auto u = [&](int i) { return __float_as_uint(p[i]); };
+        a = make_uint4(u(0), u(1), u(2), u(3));
+        b = make_uint4(u(4), u(5), u(6), u(7));
+    }
+};
+
+// ALIGNED: sources at multiples of 16 bytes, rows of codes at multiples of 4; otherwise element by element, byte by byte.
+template <typename Eight, bool ALIGNED>
+__global__ void __launch_bounds__(kThreads) pagedCachingFp4Kernel(QuantArgs a) {
+    const uint32_t first = blockIdx.x * a.block_tokens;
+    const uint32_t lanes = min(a.block_tokens, a.num_tokens - first) * a.token_lanes;
+    // token_lanes is a multiple of four (sizes are of 32), so the four lanes of a group stay or leave together
+    for (uint32_t at = threadIdx.x; at < lanes; at += kThreads) {
+        const uint32_t t = at / a.token_lanes;
+        uint32_t u = at - t * a.token_lanes;
+        const bool value = u >= a.k_lanes;
+        u -= value ? a.k_lanes : 0;
+        const Side &side = value ? a.v : a.k;
+        const uint32_t head = u / side.lanes_per_row, chunk = u - head * side.lanes_per_row;
+        const uint32_t token = first + t;
+        const int64_t slot = a.slot_mapping[token];
+        const auto *source = static_cast<const typename Eight::Element *>(side.source) + token * side.token_stride
+                           + head * side.head_stride + chunk * kPerLane;
+        Eight eight;
+        if constexpr (ALIGNED) {
+            eight.load(source);
+        } else {
+            eight.loadEach(source);
+        }
+        // a negative slot is padding; one past the pool is dropped
+        const bool held = slot >= 0 && slot < a.num_slots;
+        const uint32_t scale = mx::scaleFor(__uint_as_float(groupMax(eight.top())));
+        const uint32_t codes = scale == 0xff ? 0 : eight.codes(mx::scaleOf(scale));
+        if (held) {
+            const int64_t page = a.block_shift >= 0 ? slot >> a.block_shift : slot / a.block_size;
+            const int64_t row = slot - page * a.block_size;
+            uint8_t *to = side.codes + page * side.code_block + head * side.code_head + row * side.code_row + chunk * 4;
+            if constexpr (ALIGNED) {
+                storeStreamed(to, codes);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    to[i] = static_cast<uint8_t>(codes >> (8 * i));
+                }
+            }
+            if ((chunk & 3) == 0) {
+                side.scales[page * side.scale_block + head * side.scale_head + row * side.scale_row + (chunk >> 2)] =
+                    static_cast<uint8_t>(scale);
+            }
+        }
+    }
+}
+
+Side sideOf(void *codes, void *scales, const void *source, const fp4::PoolStrides &c, const fp4::PoolStrides &s,
+            ptrdiff_t token_stride, ptrdiff_t head_stride, size_t size) {
+    return Side{static_cast<uint8_t *>(codes), static_cast<uint8_t *>(scales), source, c.block, c.head, c.row,
+                s.block, s.head, s.row, token_stride, head_stride, static_cast<uint32_t>(size / kPerLane)};
+}
+
+} // namespace
+
+struct Descriptor::Opaque {};
+
+Descriptor::~Descriptor() { delete _opaque; }
+
+infiniStatus_t Descriptor::create(infiniopHandle_t handle, Descriptor **desc_ptr, infiniopTensorDescriptor_t k_codes_desc,
+                                  infiniopTensorDescriptor_t v_codes_desc, infiniopTensorDescriptor_t k_scales_desc,
+                                  infiniopTensorDescriptor_t v_scales_desc, infiniopTensorDescriptor_t k_desc,
+                                  infiniopTensorDescriptor_t v_desc, infiniopTensorDescriptor_t slot_mapping_desc) {
+    auto info = PagedCachingFp4Info::create(k_codes_desc, v_codes_desc, k_scales_desc, v_scales_desc, k_desc, v_desc,
+                                            slot_mapping_desc);
+    CHECK_RESULT(info);
+    const PagedCachingFp4Info in = info.take();
+    // the kernel counts tokens, rows of a page and the lanes of a workgroup in 32 bits
+    if (in.num_tokens > 0x7fffffff || in.pool.block_size > 0x7fffffff || in.pool.num_kv_heads > 0xffff
+        || in.pool.k_size > 0xffff || in.pool.v_size > 0xffff) {
+        return INFINI_STATUS_BAD_TENSOR_SHAPE;
+    }
+    *desc_ptr = new Descriptor(new Opaque{}, in, 0, handle->device, handle->device_id);
+    return INFINI_STATUS_SUCCESS;
+}
+
+infiniStatus_t Descriptor::calculate(void *workspace, size_t workspace_size, void *k_codes, void *v_codes, void *k_scales,
+                                     void *v_scales, const void *k, const void *v, const void *slot_mapping,
+                                     void *stream_) const {
+    (void)workspace;
+    (void)workspace_size;
+    const PagedCachingFp4Info &in = _info;
+    const fp4::PoolInfo &pool = in.pool;
+    if (in.num_tokens == 0 || pool.num_kv_heads == 0 || pool.num_blocks == 0 || pool.block_size == 0
+        || pool.k_size + pool.v_size == 0) {
+        return INFINI_STATUS_SUCCESS;
+    }
+    const bool keys = pool.k_size > 0, values = pool.v_size > 0;
+    if (slot_mapping == nullptr || (keys && (k_codes == nullptr || k_scales == nullptr || k == nullptr))
+        || (values && (v_codes == nullptr || v_scales == nullptr || v == nullptr))) {
+        return INFINI_STATUS_NULL_POINTER;
+    }
+    int current_device = -1;
+    if (hipGetDevice(&current_device) != hipSuccess || current_device != device_id) {
+        return INFINI_STATUS_BAD_PARAM;
+    }
+    const uint64_t es = infiniSizeOf(in.dtype);
+    auto address = [](const void *p) { return reinterpret_cast<uint64_t>(p); };
+    if ((address(k) | address(v)) % es != 0 || address(slot_mapping) % 8 != 0) {
+        return INFINI_STATUS_BAD_PARAM; // a base address that is not aligned to the element size
+    }
+
+    QuantArgs a{};
+    a.k = sideOf(k_codes, k_scales, k, pool.k_codes, pool.k_scales, in.k_token_stride, in.k_head_stride, pool.k_size);
+    a.v = sideOf(v_codes, v_scales, v, pool.v_codes, pool.v_scales, in.v_token_stride, in.v_head_stride, pool.v_size);
+    a.slot_mapping = static_cast<const int64_t *>(slot_mapping);
+    a.num_slots = static_cast<int64_t>(pool.num_blocks) * static_cast<int64_t>(pool.block_size);
+    a.num_tokens = static_cast<uint32_t>(in.num_tokens);
+    a.k_lanes = static_cast<uint32_t>(pool.num_kv_heads) * a.k.lanes_per_row;
+    a.token_lanes = a.k_lanes + static_cast<uint32_t>(pool.num_kv_heads) * a.v.lanes_per_row;
+    a.block_tokens = a.token_lanes >= kThreads ? 1 : kThreads / a.token_lanes;
+    a.block_size = static_cast<uint32_t>(pool.block_size);
+    a.block_shift = (a.block_size & (a.block_size - 1)) == 0 ? __builtin_ctz(a.block_size) : -1;
+
+    const uint64_t sources = address(k) | address(v)
+                           | (static_cast<uint64_t>(in.k_token_stride | in.k_head_stride | in.v_token_stride | in.v_head_stride) * es);
+    const bool aligned = sources % 16 == 0 && (address(k_codes) | address(v_codes)) % 4 == 0 && pool.codeRowsAligned(4);
+    const uint32_t grid = (a.num_tokens + a.block_tokens - 1) / a.block_tokens;
+    auto stream = static_cast<hipStream_t>(stream_);
+    auto launch = [&](auto eight) {
+        using Eight = decltype(eight);
+        if (aligned) {
+            pagedCachingFp4Kernel<Eight, true><<<grid, kThreads, 0, stream>>>(a);
+        } else {
+            pagedCachingFp4Kernel<Eight, false><<<grid, kThreads, 0, stream>>>(a);
+        }
+    };
+    switch (in.dtype) {
+    case INFINI_DTYPE_BF16: launch(EightBF16{}); break;
+    case INFINI_DTYPE_F16: launch(EightF16{}); break;
+    default: launch(EightF32{}); break;
+    }
+    return hipGetLastError() == hipSuccess ? INFINI_STATUS_SUCCESS : INFINI_STATUS_INTERNAL_ERROR;
+}
+
+} // namespace op::paged_caching_fp4::amd

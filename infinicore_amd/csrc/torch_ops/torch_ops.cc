@@ -42,17 +42,22 @@ using infinicore_amd::MetaKeyHash;
 struct Operator {
     int tensors;
     int device_tensor;  // the tensor that says which device (and must be on one)
-    bool has_out;       // tensors[0] is the output, allocated here where it is None
+    int outs;           // the first tensors are outputs, allocated here where they are None: 0, 1 (as the query, with the
+                        // width of tensors[3]) or 2 (tokens read out of tensors[2], tensors[3])
     bool last_optional; // the last tensor may be None
     bool keeps_scratch; // its scratch is worth keeping from call to call
+    int packed;         // elements per item of the innermost dimension of tensors[2] and [3]: 2 where a byte holds two
+    bool one_device;    // every tensor has to be on that device
 };
 constexpr Operator kOperators[] = {
-    {7, 1, true, true, true},     // paged_attention: out, q, k_cache, v_cache, block_tables, cache_lens, alibi_slopes
-    {8, 1, true, true, false},    // paged_attention_prefill: ... seq_lens, cum_seq_lens_q, alibi_slopes
-    {5, 2, false, false, false},  // paged_caching: k_cache, v_cache, k, v, slot_mapping
-    {8, 2, false, false, false},  // rope_paged_caching: ... slot_mapping, pos_ids, sin_table, cos_table
-    {10, 4, false, false, false}, // the same with q_out, q in front
-    {5, 2, false, false, false},  // kv_caching: k_cache, v_cache, k, v, past_kv_lengths
+    {7, 1, 1, true, true, 1, false},     // paged_attention: out, q, k_cache, v_cache, block_tables, cache_lens, alibi_slopes
+    {8, 1, 1, true, false, 1, false},    // paged_attention_prefill: ... seq_lens, cum_seq_lens_q, alibi_slopes
+    {5, 2, 0, false, false, 1, false},   // paged_caching: k_cache, v_cache, k, v, slot_mapping
+    {8, 2, 0, false, false, 1, false},   // rope_paged_caching: ... slot_mapping, pos_ids, sin_table, cos_table
+    {10, 4, 0, false, false, 1, false},  // the same with q_out, q in front
+    {5, 2, 0, false, false, 1, false},   // kv_caching: k_cache, v_cache, k, v, past_kv_lengths
+    {7, 4, 0, false, false, 2, true},    // paged_caching_fp4: k_codes, v_codes, k_scales, v_scales, k, v, slot_mapping
+    {7, 2, 2, false, false, 2, true},    // paged_reading_fp4: k, v, k_codes, v_codes, k_scales, v_scales, slot_mapping
 };
 constexpr int kNumOperators = sizeof(kOperators) / sizeof(kOperators[0]);
 constexpr int kMaxTensors = 10;
@@ -135,6 +140,8 @@ int callLibrary(int kind, const Entry &e, void *workspace, void *const *p, void 
     case 1: return reinterpret_cast<int (*)(V, V, size_t, V, C, C, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], stream);
     case 3: return reinterpret_cast<int (*)(V, V, size_t, V, V, C, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], stream);
     case 4: return reinterpret_cast<int (*)(V, V, size_t, V, C, V, V, C, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], stream);
+    case 6: return reinterpret_cast<int (*)(V, V, size_t, V, V, V, V, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], stream);
+    case 7: return reinterpret_cast<int (*)(V, V, size_t, V, V, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], stream);
     default: return reinterpret_cast<int (*)(V, V, size_t, V, V, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], stream);
     }
 }
@@ -184,8 +191,47 @@ PyObject *setup(PyObject *, PyObject *args) {
     Py_RETURN_NONE;
 }
 
-// call(operator, number, make, tensor or None ...) -> the first tensor, or the status as a number where it says failure
-// `number` is the scale or the algorithm; make(number, *tensors) returns a plan, called when there is none yet.
+// The tensors a call allocates: as many as it has outputs.
+struct Allocated {
+    at::Tensor tensor[2];
+};
+
+// The outputs of a call that were not handed over, by the shapes of its other tensors; false with an error set.
+bool allocateOuts(const Operator &op, double number, const at::Tensor **t, Allocated &made) {
+    const at::Tensor &on = *t[op.device_tensor];
+    if (op.outs == 1 && t[0] == nullptr) {
+        if (t[3]->dim() == 0) {
+            PyErr_SetString(PyExc_IndexError, op.packed == 2 ? "v_codes has no dimensions" : "v_cache has no dimensions");
+            return false;
+        }
+        // (a query without dimensions is refused by the operator, with its status)
+        c10::DimVector shape(on.sizes().begin(), on.sizes().begin() + std::max<int64_t>(on.dim() - 1, 0));
+        shape.push_back(t[3]->size(-1) * op.packed);
+        made.tensor[0] = at::empty(shape, at::TensorOptions().dtype(on.scalar_type()).device(on.device()));
+        t[0] = &made.tensor[0];
+    }
+    if (op.outs == 2 && (t[0] == nullptr || t[1] == nullptr)) {
+        const at::Tensor &slots = *t[op.tensors - 1];
+        if (t[2]->dim() != 4 || t[3]->dim() != 4 || slots.dim() != 1) {
+            PyErr_SetString(PyExc_IndexError, "codes of four dimensions and slots of one are expected");
+            return false;
+        }
+        for (int i = 0; i < 2; ++i) {
+            if (t[i] == nullptr) {
+                const at::Tensor &codes = *t[2 + i];
+                made.tensor[i] = at::empty({slots.size(0), codes.size(1), codes.size(3) * op.packed},
+                                           at::TensorOptions().dtype(static_cast<at::ScalarType>(static_cast<int>(number))).device(on.device()));
+                t[i] = &made.tensor[i];
+            }
+        }
+    }
+    return true;
+}
+
+// call(operator, number, make, tensor or None ...) -> the output or outputs (without any, the first tensor), or the status
+// as a number where it says failure
+// `number` is the scale or the algorithm, or the type of the outputs that are allocated here (torch's number of it);
+// make(number, *tensors) returns a plan, called when there is none yet.
 PyObject *call(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     const long kind = nargs >= 3 ? PyLong_AsLong(args[0]) : -1;
@@ -203,7 +249,7 @@ PyObject *call(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const at::Tensor *t[kMaxTensors];
     for (int i = 0; i < op.tensors; ++i) {
         PyObject *x = args[3 + i];
-        if (x == Py_None && ((i == 0 && op.has_out) || (i == op.tensors - 1 && op.last_optional))) {
+        if (x == Py_None && (i < op.outs || (i == op.tensors - 1 && op.last_optional))) {
             t[i] = nullptr;
         } else if (THPVariable_Check(x)) {
             t[i] = &THPVariable_Unpack(x);
@@ -218,17 +264,17 @@ PyObject *call(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         return nullptr;
     }
     const c10::DeviceIndex device = on.device().index();
-    at::Tensor allocated;
-    if (op.has_out && t[0] == nullptr) {
-        if (t[3]->dim() == 0) {
-            PyErr_SetString(PyExc_IndexError, "v_cache has no dimensions");
-            return nullptr;
+    if (op.one_device) {
+        for (int i = 0; i < op.tensors; ++i) {
+            if (t[i] != nullptr && t[i]->device() != on.device()) {
+                PyErr_SetString(PyExc_ValueError, "all tensors of a call have to be on one device");
+                return nullptr;
+            }
         }
-        // (a query without dimensions is refused by the operator, with its status)
-        c10::DimVector shape(on.sizes().begin(), on.sizes().begin() + std::max<int64_t>(on.dim() - 1, 0));
-        shape.push_back(t[3]->size(-1));
-        allocated = at::empty(shape, at::TensorOptions().dtype(on.scalar_type()).device(on.device()));
-        t[0] = &allocated;
+    }
+    Allocated made;
+    if (!allocateOuts(op, number, t, made)) {
+        return nullptr;
     }
     const hipStream_t stream = c10::hip::getCurrentHIPStream(device).stream();
 
@@ -264,16 +310,18 @@ PyObject *call(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         for (int i = 0; i < op.tensors; ++i) {
             make_args[1 + i] = args[3 + i];
         }
-        PyObject *wrapped = nullptr;
-        if (allocated.defined()) {
-            wrapped = THPVariable_Wrap(allocated);
-            if (wrapped == nullptr) {
-                return nullptr;
+        PyObject *wrapped[2] = {nullptr, nullptr};
+        bool failed = false;
+        for (int i = 0; i < op.outs; ++i) {
+            if (made.tensor[i].defined() && !failed) {
+                wrapped[i] = THPVariable_Wrap(made.tensor[i]);
+                failed = wrapped[i] == nullptr;
+                make_args[1 + i] = wrapped[i];
             }
-            make_args[1] = wrapped;
         }
-        PyObject *plan = PyObject_Vectorcall(args[2], make_args.data(), make_args.size(), nullptr);
-        Py_XDECREF(wrapped);
+        PyObject *plan = failed ? nullptr : PyObject_Vectorcall(args[2], make_args.data(), make_args.size(), nullptr);
+        Py_XDECREF(wrapped[0]);
+        Py_XDECREF(wrapped[1]);
         if (plan == nullptr) {
             return nullptr;
         }
@@ -317,21 +365,29 @@ PyObject *call(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (!g_retired.empty()) {
         closeRetired();
     }
-    PyObject *first;
-    if (allocated.defined()) {
-        first = THPVariable_Wrap(allocated);
-        if (first == nullptr) {
-            return nullptr;
-        }
-    } else {
-        first = args[3];
-        Py_INCREF(first);
-    }
     if (status != 0) {
-        Py_DECREF(first);
         return PyLong_FromLong(status);
     }
-    return first;
+    PyObject *result[2] = {nullptr, nullptr};
+    for (int i = 0; i < std::max(op.outs, 1); ++i) {
+        if (made.tensor[i].defined()) {
+            result[i] = THPVariable_Wrap(made.tensor[i]);
+            if (result[i] == nullptr) {
+                Py_XDECREF(result[0]);
+                return nullptr;
+            }
+        } else {
+            result[i] = args[3 + i];
+            Py_INCREF(result[i]);
+        }
+    }
+    if (op.outs < 2) {
+        return result[0];
+    }
+    PyObject *both = PyTuple_Pack(2, result[0], result[1]);
+    Py_DECREF(result[0]);
+    Py_DECREF(result[1]);
+    return both;
     END_HANDLE_TH_ERRORS
 }
 

@@ -87,6 +87,8 @@ target("infiniop-amd")
     add_files("../src/infiniop/devices/amd/*.cc")
     add_files("../src/infiniop/ops/kv_caching/amd/*.hip")
     add_files("../src/infiniop/ops/rope_paged_caching/amd/*.hip")
+    add_files("../src/infiniop/ops/paged_caching_fp4/amd/*.hip")
+    add_files("../src/infiniop/ops/paged_reading_fp4/amd/*.hip")
     -- the scatter kernel gets its first 14 argument words in scalar registers at wavefront start
     add_files("../src/infiniop/ops/paged_caching/amd/*.hip", {cxflags = {"-mllvm", "-amdgpu-kernarg-preload-count=14"}})
     -- the attention kernels keep their matrix-instruction accumulators in ordinary vector registers

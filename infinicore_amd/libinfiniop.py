@@ -183,6 +183,16 @@ def _open():
     _declare(op, "infiniopGetKVCachingWorkspaceSize", [D, POINTER(c_size_t)])
     _declare(op, "infiniopKVCaching", [D, vp, c_size_t, vp, vp, vp, vp, vp, vp])
     _declare(op, "infiniopDestroyKVCachingDescriptor", [D])
+
+    # ---- the pool held in 4 bits ----
+    _declare(op, "infiniopCreatePagedCachingFp4Descriptor", [infiniopHandle_t, POINTER(D)] + [T] * 7)
+    _declare(op, "infiniopGetPagedCachingFp4WorkspaceSize", [D, POINTER(c_size_t)])
+    _declare(op, "infiniopPagedCachingFp4", [D, vp, c_size_t] + [vp] * 8)
+    _declare(op, "infiniopDestroyPagedCachingFp4Descriptor", [D])
+    _declare(op, "infiniopCreatePagedReadingFp4Descriptor", [infiniopHandle_t, POINTER(D)] + [T] * 7)
+    _declare(op, "infiniopGetPagedReadingFp4WorkspaceSize", [D, POINTER(c_size_t)])
+    _declare(op, "infiniopPagedReadingFp4", [D, vp, c_size_t] + [vp] * 8)
+    _declare(op, "infiniopDestroyPagedReadingFp4Descriptor", [D])
     return rt, op
 
 

@@ -1,4 +1,5 @@
-"""``paged_attention`` / ``paged_attention_prefill`` / ``paged_caching`` on torch CUDA tensors, executed by ``libinfiniop.so``.
+"""``paged_attention`` / ``paged_attention_prefill`` / ``paged_caching`` on torch CUDA tensors, executed by ``libinfiniop.so``;
+beside them the same family over a pool held in 4 bits (``..._fp4``).
 
 Argument order and meaning are those of the reference's Python operators
 (``python/infinicore/ops/paged_attention.py:5-40``, ``python/infinicore/ops/paged_attention_prefill.py:5-45``,
@@ -55,9 +56,10 @@ def _load_native():
 
 _native = _load_native()
 # the operators by number, as csrc/torch_ops/torch_ops.cc lists them
-(_PAGED_ATTENTION, _PAGED_ATTENTION_PREFILL, _PAGED_CACHING, _ROPE_PAGED_CACHING, _ROPE_QK_PAGED_CACHING, _KV_CACHING) = range(6)
+(_PAGED_ATTENTION, _PAGED_ATTENTION_PREFILL, _PAGED_CACHING, _ROPE_PAGED_CACHING, _ROPE_QK_PAGED_CACHING, _KV_CACHING,
+ _PAGED_CACHING_FP4, _PAGED_READING_FP4) = range(8)
 _RUN = ("infiniopPagedAttention", "infiniopPagedAttentionPrefill", "infiniopPagedCaching", "infiniopRoPEPagedCaching",
-        "infiniopRoPEQKPagedCaching", "infiniopKVCaching")
+        "infiniopRoPEQKPagedCaching", "infiniopKVCaching", "infiniopPagedCachingFp4", "infiniopPagedReadingFp4")
 _native.setup(tuple(ctypes.cast(getattr(LIBINFINIOP, name), c_void_p).value for name in _RUN),
               ctypes.cast(lib.LIBINFINIRT.infinirtSetDevice, c_void_p).value, int(InfiniDevice.AMD), _PLAN_CACHE_CAPACITY)
 
@@ -145,9 +147,19 @@ def _make_kv_caching(_, *tensors):
                  "infiniopDestroyKVCachingDescriptor", tensors[2].device, tensors)
 
 
+def _make_paged_caching_fp4(_, *tensors):
+    return _plan("infiniopCreatePagedCachingFp4Descriptor", "infiniopGetPagedCachingFp4WorkspaceSize",
+                 "infiniopDestroyPagedCachingFp4Descriptor", tensors[4].device, tensors)
+
+
+def _make_paged_reading_fp4(_, *tensors):
+    return _plan("infiniopCreatePagedReadingFp4Descriptor", "infiniopGetPagedReadingFp4WorkspaceSize",
+                 "infiniopDestroyPagedReadingFp4Descriptor", tensors[2].device, tensors)
+
+
 def _call(operator, number, make, *tensors):
     result = _native.call(operator, number, make, *tensors)
-    if type(result) is int:  # a status; otherwise the first tensor
+    if type(result) is int:  # a status; otherwise the output, both outputs or the first tensor
         check_error(result, _RUN[operator])
     return result
 
@@ -205,3 +217,31 @@ def kv_caching(k_cache, v_cache, k, v, past_kv_lengths):
     the caches (argument order of the reference's infiniopKVCaching, include/infiniop/ops/kv_caching.h:8-29)."""
     _call(_KV_CACHING, 0, _make_kv_caching, k_cache, v_cache, k, v, past_kv_lengths)
     return k_cache, v_cache
+
+
+# ---- the pool held in 4 bits ----
+# k_codes / v_codes [num_blocks, num_kv_heads, block_size, d / 2] uint8: two e2m1 codes per byte, the even element in the low
+# half; k_scales / v_scales [num_blocks, num_kv_heads, block_size, d / 32] uint8: an exponent (bias 127) for each 32 elements.
+# Zeros everywhere are a pool of zeros. The format is written out in include/infiniop/ops/paged_caching_fp4.h.
+
+# torch's numbers of the types that tokens are read back as
+_READ_TYPES = {torch.float16: 5, torch.float32: 6, torch.bfloat16: 15}
+
+
+def paged_caching_fp4(k_codes, v_codes, k_scales, v_scales, k, v, slot_mapping):
+    """Quantise ``k`` / ``v`` [num_tokens, num_kv_heads, d] (fp16, bf16 or fp32) to 4 bits and scatter them into the pools
+    in place, a negative slot being padding; returns the four pools. The 4-bit counterpart of ``paged_caching``."""
+    _call(_PAGED_CACHING_FP4, 0, _make_paged_caching_fp4, k_codes, v_codes, k_scales, v_scales, k, v, slot_mapping)
+    return k_codes, v_codes, k_scales, v_scales
+
+
+def paged_reading_fp4(k_codes, v_codes, k_scales, v_scales, slot_mapping, *, dtype=None, k=None, v=None):
+    """Read the tokens of ``slot_mapping`` out of a pool held in 4 bits, as the values they stand for; returns ``(k, v)``
+    [num_tokens, num_kv_heads, d], of ``dtype`` (default bfloat16) where they are allocated here. A negative slot reads as
+    zeros. ``k.view(-1, block_size, num_kv_heads, d).transpose(1, 2)`` is a pool that the 16-bit operators take."""
+    if dtype is None:
+        dtype = next((t.dtype for t in (k, v) if t is not None), torch.bfloat16)
+    if dtype not in _READ_TYPES:
+        raise ValueError(f"tokens are read back as float16, bfloat16 or float32, not {dtype}")
+    return _call(_PAGED_READING_FP4, _READ_TYPES[dtype], _make_paged_reading_fp4, k, v, k_codes, v_codes, k_scales, v_scales,
+                 slot_mapping)
