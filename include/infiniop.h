@@ -6,6 +6,7 @@
 #include "infiniop/operator_descriptor.h"
 #include "infiniop/ops/kv_caching.h"
 #include "infiniop/ops/paged_attention.h"
+#include "infiniop/ops/paged_attention_fp4.h"
 #include "infiniop/ops/paged_attention_prefill.h"
 #include "infiniop/ops/paged_caching.h"
 #include "infiniop/ops/paged_caching_fp4.h"

@@ -1,0 +1,71 @@
+/*
+ * Paged attention, decode step, over a pool held in 4 bits: one query token per sequence against that sequence's cached K/V.
+ * The pool is the one that infiniopPagedCachingFp4 writes; its header describes the format.
+ *
+ * Tensors (strides in elements; the innermost dimension packed everywhere):
+ *   out           [num_seqs, num_heads, head_size]   F16 | BF16
+ *   q             [num_seqs, num_heads, head_size]   same dtype
+ *   k_codes       [num_blocks, num_kv_heads, block_size, head_size / 2]   U8, strides of dims 0-2 multiples of 16
+ *   v_codes       like k_codes
+ *   k_scales      [num_blocks, num_kv_heads, block_size, head_size / 32]  U8, any strides on dims 0-2
+ *   v_scales      like k_scales
+ *   block_tables  [num_seqs or more, max_blocks_per_seq]  I64 | I32 | U32
+ *   seq_lens      [num_seqs]                              same index dtype; tokens of each sequence, the current one included
+ *   alibi_slopes  [num_heads or more] F32, or NULL
+ *   head_size 64, 128, 192 or 256; block_size any; num_heads a multiple of num_kv_heads, query head h reads KV head
+ *   h / (num_heads / num_kv_heads).
+ *
+ * out[s, h] = sum over t < seq_lens[s] of p_t v_t, p = softmax(scale * q . k_t + alibi[h] * (t - (seq_lens[s] - 1))).
+ * A sequence of no tokens (seq_lens[s] <= 0) leaves its rows of out as they were; lengths beyond what the block table can
+ * hold are cut to that, page ids outside the pool are forced into it. Rows of a page behind a sequence's end have no
+ * part in the result, whatever they hold. Values are exact as stored for scales of 0.5 * 2^-23 .. 2^13 as written by
+ * infiniopPagedCachingFp4; the products with V are taken in fp16, so that values beyond its range (pools from elsewhere)
+ * count as infinite or zero.
+ */
+#ifndef INFINICORE_AMD_INFINIOP_PAGED_ATTENTION_FP4_H
+#define INFINICORE_AMD_INFINIOP_PAGED_ATTENTION_FP4_H
+
+#include "../operator_descriptor.h"
+
+typedef struct InfiniopDescriptor *infiniopPagedAttentionFp4Descriptor_t;
+
+__INFINI_C __export infiniStatus_t infiniopCreatePagedAttentionFp4Descriptor(
+    infiniopHandle_t handle,
+    infiniopPagedAttentionFp4Descriptor_t *desc_ptr,
+    infiniopTensorDescriptor_t out_desc,
+    infiniopTensorDescriptor_t q_desc,
+    infiniopTensorDescriptor_t k_codes_desc,
+    infiniopTensorDescriptor_t v_codes_desc,
+    infiniopTensorDescriptor_t k_scales_desc,
+    infiniopTensorDescriptor_t v_scales_desc,
+    infiniopTensorDescriptor_t block_tables_desc,
+    infiniopTensorDescriptor_t seq_lens_desc,
+    infiniopTensorDescriptor_t alibi_slopes_desc, /* NULL = no ALiBi */
+    float scale);
+
+/* Bytes of scratch that a call needs; its content does not matter. Two calls that overlap in time need two. */
+__INFINI_C __export infiniStatus_t infiniopGetPagedAttentionFp4WorkspaceSize(
+    infiniopPagedAttentionFp4Descriptor_t desc,
+    size_t *size);
+
+/* Enqueues on `stream`, allocates nothing and waits for nothing. BAD_PARAM where the calling thread's current device is not
+ * the descriptor's, or where codes do not begin at a multiple of 16 bytes. */
+__INFINI_C __export infiniStatus_t infiniopPagedAttentionFp4(
+    infiniopPagedAttentionFp4Descriptor_t desc,
+    void *workspace,
+    size_t workspace_size,
+    void *out,
+    const void *q,
+    const void *k_codes,
+    const void *v_codes,
+    const void *k_scales,
+    const void *v_scales,
+    const void *block_tables,
+    const void *seq_lens,
+    const void *alibi_slopes,
+    void *stream);
+
+__INFINI_C __export infiniStatus_t infiniopDestroyPagedAttentionFp4Descriptor(
+    infiniopPagedAttentionFp4Descriptor_t desc);
+
+#endif /* INFINICORE_AMD_INFINIOP_PAGED_ATTENTION_FP4_H */

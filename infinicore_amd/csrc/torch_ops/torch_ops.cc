@@ -58,6 +58,8 @@ constexpr Operator kOperators[] = {
     {5, 2, 0, false, false, 1, false},   // kv_caching: k_cache, v_cache, k, v, past_kv_lengths
     {7, 4, 0, false, false, 2, true},    // paged_caching_fp4: k_codes, v_codes, k_scales, v_scales, k, v, slot_mapping
     {7, 2, 2, false, false, 2, true},    // paged_reading_fp4: k, v, k_codes, v_codes, k_scales, v_scales, slot_mapping
+    {9, 1, 1, true, false, 2, true},     // paged_attention_fp4: out, q, k_codes, v_codes, k_scales, v_scales, block_tables,
+                                         // cache_lens, alibi_slopes
 };
 constexpr int kNumOperators = sizeof(kOperators) / sizeof(kOperators[0]);
 constexpr int kMaxTensors = 10;
@@ -142,6 +144,7 @@ int callLibrary(int kind, const Entry &e, void *workspace, void *const *p, void 
     case 4: return reinterpret_cast<int (*)(V, V, size_t, V, C, V, V, C, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], stream);
     case 6: return reinterpret_cast<int (*)(V, V, size_t, V, V, V, V, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], stream);
     case 7: return reinterpret_cast<int (*)(V, V, size_t, V, V, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], stream);
+    case 8: return reinterpret_cast<int (*)(V, V, size_t, V, C, C, C, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], stream);
     default: return reinterpret_cast<int (*)(V, V, size_t, V, V, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], stream);
     }
 }

@@ -193,6 +193,10 @@ def _open():
     _declare(op, "infiniopGetPagedReadingFp4WorkspaceSize", [D, POINTER(c_size_t)])
     _declare(op, "infiniopPagedReadingFp4", [D, vp, c_size_t] + [vp] * 8)
     _declare(op, "infiniopDestroyPagedReadingFp4Descriptor", [D])
+    _declare(op, "infiniopCreatePagedAttentionFp4Descriptor", [infiniopHandle_t, POINTER(D)] + [T] * 9 + [c_float])
+    _declare(op, "infiniopGetPagedAttentionFp4WorkspaceSize", [D, POINTER(c_size_t)])
+    _declare(op, "infiniopPagedAttentionFp4", [D, vp, c_size_t] + [vp] * 10)
+    _declare(op, "infiniopDestroyPagedAttentionFp4Descriptor", [D])
     return rt, op
 
 

@@ -57,9 +57,10 @@ def _load_native():
 _native = _load_native()
 # the operators by number, as csrc/torch_ops/torch_ops.cc lists them
 (_PAGED_ATTENTION, _PAGED_ATTENTION_PREFILL, _PAGED_CACHING, _ROPE_PAGED_CACHING, _ROPE_QK_PAGED_CACHING, _KV_CACHING,
- _PAGED_CACHING_FP4, _PAGED_READING_FP4) = range(8)
+ _PAGED_CACHING_FP4, _PAGED_READING_FP4, _PAGED_ATTENTION_FP4) = range(9)
 _RUN = ("infiniopPagedAttention", "infiniopPagedAttentionPrefill", "infiniopPagedCaching", "infiniopRoPEPagedCaching",
-        "infiniopRoPEQKPagedCaching", "infiniopKVCaching", "infiniopPagedCachingFp4", "infiniopPagedReadingFp4")
+        "infiniopRoPEQKPagedCaching", "infiniopKVCaching", "infiniopPagedCachingFp4", "infiniopPagedReadingFp4",
+        "infiniopPagedAttentionFp4")
 _native.setup(tuple(ctypes.cast(getattr(LIBINFINIOP, name), c_void_p).value for name in _RUN),
               ctypes.cast(lib.LIBINFINIRT.infinirtSetDevice, c_void_p).value, int(InfiniDevice.AMD), _PLAN_CACHE_CAPACITY)
 
@@ -157,6 +158,11 @@ def _make_paged_reading_fp4(_, *tensors):
                  "infiniopDestroyPagedReadingFp4Descriptor", tensors[2].device, tensors)
 
 
+def _make_paged_attention_fp4(scale, *tensors):
+    return _plan("infiniopCreatePagedAttentionFp4Descriptor", "infiniopGetPagedAttentionFp4WorkspaceSize",
+                 "infiniopDestroyPagedAttentionFp4Descriptor", tensors[1].device, tensors[:-1], scale, optional=tensors[-1:])
+
+
 def _call(operator, number, make, *tensors):
     result = _native.call(operator, number, make, *tensors)
     if type(result) is int:  # a status; otherwise the output, both outputs or the first tensor
@@ -245,3 +251,11 @@ def paged_reading_fp4(k_codes, v_codes, k_scales, v_scales, slot_mapping, *, dty
         raise ValueError(f"tokens are read back as float16, bfloat16 or float32, not {dtype}")
     return _call(_PAGED_READING_FP4, _READ_TYPES[dtype], _make_paged_reading_fp4, k, v, k_codes, v_codes, k_scales, v_scales,
                  slot_mapping)
+
+
+def paged_attention_fp4(q, k_codes, v_codes, k_scales, v_scales, block_tables, cache_lens, alibi_slopes=None,
+                        scale: float = 1.0, *, out=None):
+    """Decode attention of one query token per sequence over a pool held in 4 bits; returns ``out``. The 4-bit counterpart of
+    ``paged_attention``: heads of 64, 128, 192 or 256, keys and values of one size."""
+    return _call(_PAGED_ATTENTION_FP4, scale, _make_paged_attention_fp4, out, q, k_codes, v_codes, k_scales, v_scales,
+                 block_tables, cache_lens, alibi_slopes)

@@ -19,7 +19,7 @@ def quantise(x):
     exponent = torch.where(top == 0, -1000, exponent)
     s = (exponent - 2).clamp(-23, 13)
     a = (torch.where(finite[..., None], g, 0.0).abs() / torch.pow(2.0, s.double())[..., None]).clamp(max=6.0)
-    distance = (a[..., None] - MAGNITUDES).abs()
+    distance = (a[..., None] - MAGNITUDES.to(x.device)).abs()
     nearest = distance.amin(-1, keepdim=True)
     even_first = torch.tensor([0, 2, 4, 6, 1, 3, 5, 7])
     code = even_first[(distance[..., even_first] == nearest).int().argmax(-1)]
@@ -32,7 +32,7 @@ def quantise(x):
 def values(codes, scales):
     """What codes [.., n / 2] under scales [.., n / 32] stand for, float64 [.., n]."""
     c = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).long()
-    v = MAGNITUDES[c & 7] * torch.where(c >= 8, -1.0, 1.0).double()
+    v = MAGNITUDES.to(codes.device)[c & 7] * torch.where(c >= 8, -1.0, 1.0).double()
     unit = torch.pow(2.0, scales.double() - 127).masked_fill(scales == 255, math.nan)
     return v * unit.repeat_interleave(GROUP, dim=-1)
 
@@ -45,21 +45,52 @@ def sequence(codes, scales, pages, tokens):
 
 def attention(q, k, v, scale, last, slopes=None):
     """q [n, heads, d] over k, v [KV heads, tokens, d]: row j sees tokens 0 .. last[j] (none where last[j] < 0: the row is
-    NaN, to be left out by the caller). A token that a row does not see has no part in it, whatever it holds."""
+    NaN, to be left out by the caller). A token that a row does not see has no part in it, whatever it holds.
+    Returns the outputs, and how far a kernel of the kind tested may be off before it rounds them (`allowed`)."""
     n, heads, d = q.shape
+    tokens = k.shape[1]
     group = heads // k.shape[0]
-    out = torch.full((n, heads, v.shape[-1]), math.nan, dtype=torch.float64)
-    for j in range(n):
-        t = int(last[j]) + 1
-        if t <= 0:
-            continue
-        for h in range(heads):
-            s = (k[h // group, :t] @ q[j, h].double()) * scale
-            if slopes is not None:
-                s = s + slopes[h].double() * (torch.arange(t, dtype=torch.float64) - last[j])
-            p = torch.exp(s - s.max())
-            out[j, h] = (p / p.sum()) @ v[h // group, :t]
-    return out
+    x = q.double()
+    sees = torch.arange(tokens, device=q.device)[None, :] <= torch.as_tensor(last, device=q.device)[:, None]
+    out = torch.full((n, heads, v.shape[-1]), math.nan, dtype=torch.float64, device=q.device)
+    allowed = torch.zeros_like(out)
+    rows = sees.any(-1)
+    for h in range(heads):
+        kh, vh = k[h // group], v[h // group]
+        s = (x[:, h] @ kh.T) * scale
+        if slopes is not None:
+            s = s + slopes[h].double() * (torch.arange(tokens, device=q.device)[None, :] - torch.as_tensor(last, device=q.device)[:, None])
+        s = torch.where(sees, s, -math.inf)
+        p = torch.softmax(s, -1)
+        finite = torch.isfinite(vh)
+        o = p @ torch.where(finite, vh, 0.0)
+        o = o + torch.where(sees.double() @ (~finite).double() > 0, math.nan, 0.0)  # a value that a row sees and is not finite
+        out[rows, h] = o[rows]
+        allowed[rows, h] = _allowed(x[:, h], kh, vh, s, p, scale, sees)[rows]
+    return out, allowed
+
+
+def _allowed(x, k, v, s, p, scale, sees):
+    """Before the outputs are rounded. Scores are fp32 sums of d exact products of up to sum |q| |k|, each addition rounded
+    (2^-24), the sum times the scale, a bias and log2(e) (four more roundings of the score's size); exp2 is good to 2^-22 of its
+    value. An error of e in a score is one of e in a probability's logarithm. Probabilities go to the matrix unit in fp16: 2^-11
+    of their value, and below 2^-14 half a step of 2^-24, against a largest one of at least 1; the denominator sums them in
+    fp32 unrounded (tokens additions, in at most 64 lanes and partial results: 2^-24 each over tokens / 16)."""
+    d, tokens = k.shape[-1], k.shape[0]
+    magnitude = (x.abs() @ torch.nan_to_num(k).abs().T * abs(scale)).masked_fill(~sees, 0.0).amax(-1)
+    score = torch.where(sees, torch.nan_to_num(s.abs(), posinf=0.0), 0.0).amax(-1)
+    e = magnitude * (d + 2) * 2.0 ** -24 + score * 4 * 2.0 ** -24 + 2.0 ** -22
+    relative = 2 * e + 2.0 ** -11 + (tokens / 16 + 16) * 2.0 ** -24
+    w = torch.nan_to_num(v).abs()
+    return torch.nan_to_num(p) @ w * relative[:, None] + (sees.double() @ w) * 2.0 ** -25
+
+
+def off_by(got, want, allowed):
+    """The largest excess of |got - want| over what is allowed and the one rounding of the outputs, in units of that sum."""
+    half = torch.finfo(got.dtype).eps / 2
+    least = {torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}[got.dtype]  # half a step of fp16's smallest values
+    bound = want.abs() * half + allowed * (1 + half) + least
+    return ((got.double() - want).abs() / bound.clamp(min=1e-300)).max().item() if got.numel() else 0.0
 
 
 def make_pool(seed, blocks, heads, page, size, *, spread=1.0):
