@@ -8,6 +8,7 @@
 #include "infiniop/ops/paged_attention.h"
 #include "infiniop/ops/paged_attention_fp4.h"
 #include "infiniop/ops/paged_attention_prefill.h"
+#include "infiniop/ops/paged_attention_prefill_fp4.h"
 #include "infiniop/ops/paged_caching.h"
 #include "infiniop/ops/paged_caching_fp4.h"
 #include "infiniop/ops/paged_reading_fp4.h"

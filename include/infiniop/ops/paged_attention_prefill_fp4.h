@@ -1,0 +1,73 @@
+/*
+ * Paged attention of runs of new tokens (prefill, chunks of one, drafted tokens) over a pool held in 4 bits. The pool is the one
+ * that infiniopPagedCachingFp4 writes; its header describes the format. The new tokens' own keys and values are in it.
+ *
+ * Tensors (strides in elements; the innermost dimension packed everywhere):
+ *   out             [total_q_tokens, num_heads, head_size]   F16 | BF16
+ *   q               [total_q_tokens, num_heads, head_size]   same dtype, the new tokens of all sequences back to back
+ *   k_codes         [num_blocks, num_kv_heads, block_size, head_size / 2]   U8, strides of dims 0-2 multiples of 16
+ *   v_codes         like k_codes
+ *   k_scales        [num_blocks, num_kv_heads, block_size, head_size / 32]  U8, any strides on dims 0-2
+ *   v_scales        like k_scales
+ *   block_tables    [num_seqs or more, max_blocks_per_seq]  I64 | I32 | U32
+ *   seq_lens        [num_seqs]      same index dtype; tokens of each sequence, the new ones included
+ *   cum_seq_lens_q  [num_seqs + 1]  same index dtype; prefix sums of the new tokens
+ *   alibi_slopes    [num_heads or more] F32, or NULL
+ *   head_size 64, 128, 192 or 256; block_size any; num_heads a multiple of num_kv_heads, query head h reads KV head
+ *   h / (num_heads / num_kv_heads).
+ *
+ * Row i = cum_seq_lens_q[s] + j belongs to sequence s, stands at position pos = seq_lens[s] - (its new tokens) + j, and
+ *   out[i, h] = sum over t <= pos of p_t v_t, p = softmax(scale * q . k_t + alibi[h] * (t - pos)).
+ * Rows that belong to nobody and rows that see nothing (pos < 0) are left as they were. Ranges are clipped to the operands:
+ * rows to q's, positions to what the block table can hold, page ids to the pool. A token that a row does not see has no
+ * part in that row, whatever it holds, NaN included. Values as for infiniopPagedAttentionFp4.
+ */
+#ifndef INFINICORE_AMD_INFINIOP_PAGED_ATTENTION_PREFILL_FP4_H
+#define INFINICORE_AMD_INFINIOP_PAGED_ATTENTION_PREFILL_FP4_H
+
+#include "../operator_descriptor.h"
+
+typedef struct InfiniopDescriptor *infiniopPagedAttentionPrefillFp4Descriptor_t;
+
+__INFINI_C __export infiniStatus_t infiniopCreatePagedAttentionPrefillFp4Descriptor(
+    infiniopHandle_t handle,
+    infiniopPagedAttentionPrefillFp4Descriptor_t *desc_ptr,
+    infiniopTensorDescriptor_t out_desc,
+    infiniopTensorDescriptor_t q_desc,
+    infiniopTensorDescriptor_t k_codes_desc,
+    infiniopTensorDescriptor_t v_codes_desc,
+    infiniopTensorDescriptor_t k_scales_desc,
+    infiniopTensorDescriptor_t v_scales_desc,
+    infiniopTensorDescriptor_t block_tables_desc,
+    infiniopTensorDescriptor_t seq_lens_desc,
+    infiniopTensorDescriptor_t cum_seq_lens_q_desc,
+    infiniopTensorDescriptor_t alibi_slopes_desc, /* NULL = no ALiBi */
+    float scale);
+
+/* Bytes of scratch that a call needs; its content does not matter. Two calls that overlap in time need two. */
+__INFINI_C __export infiniStatus_t infiniopGetPagedAttentionPrefillFp4WorkspaceSize(
+    infiniopPagedAttentionPrefillFp4Descriptor_t desc,
+    size_t *size);
+
+/* Enqueues on `stream`, allocates nothing and waits for nothing. BAD_PARAM where the calling thread's current device is not
+ * the descriptor's, or where codes do not begin at a multiple of 16 bytes. */
+__INFINI_C __export infiniStatus_t infiniopPagedAttentionPrefillFp4(
+    infiniopPagedAttentionPrefillFp4Descriptor_t desc,
+    void *workspace,
+    size_t workspace_size,
+    void *out,
+    const void *q,
+    const void *k_codes,
+    const void *v_codes,
+    const void *k_scales,
+    const void *v_scales,
+    const void *block_tables,
+    const void *seq_lens,
+    const void *cum_seq_lens_q,
+    const void *alibi_slopes,
+    void *stream);
+
+__INFINI_C __export infiniStatus_t infiniopDestroyPagedAttentionPrefillFp4Descriptor(
+    infiniopPagedAttentionPrefillFp4Descriptor_t desc);
+
+#endif /* INFINICORE_AMD_INFINIOP_PAGED_ATTENTION_PREFILL_FP4_H */

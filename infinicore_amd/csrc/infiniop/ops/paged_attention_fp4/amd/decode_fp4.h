@@ -125,9 +125,11 @@ template <> struct Bits<2> { using type = uint16_t; };
 template <> struct Bits<4> { using type = uint32_t; };
 template <> struct Bits<8> { typedef unsigned type __attribute__((ext_vector_type(2))); };
 template <> struct Bits<16> { typedef unsigned type __attribute__((ext_vector_type(4))); };
-template <int BYTES>
-__device__ __forceinline__ void loadOnce(const char *p, uint32_t *to) {
-    const auto v = __builtin_nontemporal_load(reinterpret_cast<const typename Bits<BYTES>::type *>(p));
+// ONCE: past the caches, for what a call reads once.
+template <int BYTES, bool ONCE = true>
+__device__ __forceinline__ void loadWords(const char *p, uint32_t *to) {
+    const auto *from = reinterpret_cast<const typename Bits<BYTES>::type *>(p);
+    const auto v = ONCE ? __builtin_nontemporal_load(from) : *from;
     if constexpr (BYTES <= 4) {
         to[0] = v;
     } else {
@@ -228,9 +230,9 @@ struct Pages {
         for (int p = 0; p < L::kPieces; ++p) {
             const int e = L::element(p, g);
             if (L::pieceWhole(p)) {
-                loadOnce<16>(codes + e / 2, &to.k[tile][4 * p]);
+                loadWords<16>(codes + e / 2, &to.k[tile][4 * p]);
             } else {
-                loadOnce<8>(codes + e / 2, &to.k[tile][4 * p]);
+                loadWords<8>(codes + e / 2, &to.k[tile][4 * p]);
             }
             to.ks[tile][p] = __builtin_nontemporal_load(reinterpret_cast<const uint8_t *>(scales + e / 32));
         }
@@ -240,9 +242,9 @@ struct Pages {
         for (int s = 0; s < L::kStrips; ++s) {
             const int d = L::column(s, c);
             if (s == 0) {
-                loadOnce<L::kStripCols / 2>(codes + d / 2, to.v[at]);
+                loadWords<L::kStripCols / 2>(codes + d / 2, to.v[at]);
             } else {
-                loadOnce<2>(codes + d / 2, &to.v[at][1]);
+                loadWords<2>(codes + d / 2, &to.v[at][1]);
             }
             to.vs[at][s] = __builtin_nontemporal_load(reinterpret_cast<const uint8_t *>(scales + d / 32));
         }

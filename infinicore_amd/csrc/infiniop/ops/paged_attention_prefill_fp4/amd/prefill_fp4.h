@@ -1,0 +1,546 @@
+// Prefill kernel over a KV pool held in 4 bits, gfx950 (CDNA4, 64-lane wavefronts), head_size = value_size = 64, 128, 192 or
+// 256.
+//
+// One 256-thread workgroup = 64 R "rows" of one (sequence, KV head); a row is a (new token, query head of the group) pair,
+// token-major. Each wavefront owns 16 R rows. The tokens that the rows may see are consumed in steps of 64 (32 at head 192
+// with R = 1): per step each wavefront loads the codes and scales of its share of the tokens, a step ahead, into registers,
+// turns them into 16-bit values between the matrix instructions of the present step (v_cvt_scalef32_pk_*, two elements per
+// instruction; K in the query's type, V in fp16, where every written value is exact) and leaves them in LDS for everybody;
+// one barrier per step. lane = 16 g + c:
+//   S[token][row] = K . Q^T   v_mfma_f32_16x16x32 (A = K out of LDS, B = Q in registers; lane holds S[16 T + 4g + 0..3][row c])
+//   causal mask (only in steps that touch the diagonal), online softmax in fp32 / log2 domain
+//   O[dim][row] += V . P      v_mfma_f32_16x16x32 (A = V by the transposing LDS read; B = P in fp16 as S came out;
+//                             lane holds O[16 e + 4g + 0..3][row c])
+//   l[row]      += 1 . P      v_mfma_f32_16x16x32
+// A value that is not finite has scale 255: it goes into LDS as zero, its token is noted, and the outputs of the rows that
+// see that token become NaN in the columns of its group; rows that do not see it are not touched by it.
+#ifndef INFINICORE_AMD_PA_PREFILL_FP4_H
+#define INFINICORE_AMD_PA_PREFILL_FP4_H
+
+#include "../../paged_attention_fp4/amd/decode_fp4.h"
+
+namespace op::paged_attention_prefill_fp4::amd {
+
+using op::paged_attention::amd::clampPage;
+using op::paged_attention::amd::f32x4;
+using op::paged_attention::amd::fastExp2;
+using op::paged_attention::amd::kLog2e;
+using op::paged_attention::amd::maxAcrossTokenGroups;
+using op::paged_attention::amd::maxOf;
+using op::paged_attention::amd::TileBF16;
+using op::paged_attention::amd::TileF16;
+using op::paged_attention::amd::waveInclusiveSum;
+using op::paged_attention::amd::waveMaxInt;
+using op::paged_attention_fp4::amd::IndexType;
+using op::paged_attention_fp4::amd::loadIndexOf;
+using op::paged_attention_fp4::amd::loadWords;
+using op::paged_attention_fp4::amd::PoolSide;
+using op::paged_attention_fp4::amd::toQueryType;
+namespace mx = device::amd::mx;
+
+constexpr int kPrefillThreads = 256;
+constexpr int kTile = 16;          // tokens of a matrix instruction
+constexpr float kLazyLog2 = 8.0f;  // how far (in powers of two) a row maximum may outgrow its reference point
+
+struct PrefillFp4Args {
+    void *out;
+    const void *q;
+    PoolSide k_codes, k_scales, v_codes, v_scales;
+    const void *block_tables;
+    const void *kv_lens;       // [num_seqs] tokens of each sequence, the new ones included
+    const void *cu_seqlens_q;  // [num_seqs + 1] prefix sums of the new tokens
+    const float *alibi_slopes; // nullptr = no ALiBi
+    IndexType index_type;
+    float scale_log2; // scale * log2(e)
+    int32_t num_seqs, total_q_tokens, num_heads, num_kv_heads;
+    int32_t group; // query heads per KV head
+    int32_t block_size;
+    int32_t num_blocks; // pool size; table entries are clamped into [0, num_blocks)
+    int32_t capacity;   // tokens that a row of the block table can hold, at most
+    bool q_aligned, out_aligned; // every row begins at a multiple of 16 bytes
+    int64_t q_stride, q_head_stride; // elements
+    int64_t o_stride, o_head_stride;
+    int64_t block_table_stride;
+};
+
+// What one sequence contributes: query token j (0 <= j < q_len) is row q_start + j of q / out and sees tokens [0, history +
+// j + 1). The row range is clipped to the query and the visible range to what the block table can hold, so that inconsistent
+// index tensors cannot reach outside the operands.
+struct Span {
+    int32_t q_start, q_len; // q_len <= 0: nothing to do
+    int32_t history;        // may be negative: the first -history query tokens then see nothing
+};
+
+__device__ __forceinline__ Span loadSpan(const PrefillFp4Args &a, int seq) {
+    int64_t q0 = loadIndexOf(a.index_type, a.cu_seqlens_q, seq), q1 = loadIndexOf(a.index_type, a.cu_seqlens_q, seq + 1);
+    const int64_t kv = loadIndexOf(a.index_type, a.kv_lens, seq);
+    const int64_t lim = int64_t(1) << 30;
+    int64_t history = kv - (q1 - q0);
+    history = history < -lim ? -lim : (history > lim ? lim : history);
+    q0 = q0 < 0 ? 0 : (q0 > a.total_q_tokens ? a.total_q_tokens : q0);
+    q1 = q1 < q0 ? q0 : (q1 > a.total_q_tokens ? a.total_q_tokens : q1);
+    return Span{static_cast<int32_t>(q0), static_cast<int32_t>(q1 - q0), static_cast<int32_t>(history)};
+}
+// Tokens that query token j may see (0 = none: its output row stays as it was).
+__device__ __forceinline__ int32_t visibleTokens(const PrefillFp4Args &a, const Span &s, int32_t j) {
+    const int32_t n = s.history + j + 1;
+    return n < 0 ? 0 : (n > a.capacity ? a.capacity : n);
+}
+
+// Which (sequence, row block) workgroup x of a KV head works on: the blocks of the last sequence first, each sequence's last
+// block first (it sees the most). False for a workgroup beyond the last block.
+__device__ __forceinline__ bool findBlock(const PrefillFp4Args &a, int lane, int block_rows, int x, int &seq, int &block, Span &span_out) {
+    for (int base = 0; base < a.num_seqs; base += 64) {
+        const int s = a.num_seqs - 1 - (base + lane);
+        int blocks = 0;
+        Span span{0, 0, 0};
+        if (s >= 0) {
+            span = loadSpan(a, s);
+            const int64_t rows = static_cast<int64_t>(span.q_len) * a.group;
+            blocks = rows > 0 ? static_cast<int>((rows + block_rows - 1) / block_rows) : 0;
+        }
+        const int sum = waveInclusiveSum(blocks);
+        const int all = __builtin_amdgcn_readlane(sum, 63);
+        if (x >= all) {
+            x -= all;
+            continue;
+        }
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > x));
+        seq = a.num_seqs - 1 - (base + at);
+        block = __builtin_amdgcn_readlane(sum, at) - 1 - x;
+        span_out.q_start = __builtin_amdgcn_readlane(span.q_start, at);
+        span_out.q_len = __builtin_amdgcn_readlane(span.q_len, at);
+        span_out.history = __builtin_amdgcn_readlane(span.history, at);
+        return true;
+    }
+    return false;
+}
+
+// A head's rows in LDS and in the lanes that fill it. A unit is what a lane converts: 32 elements (16 at head 64, so that
+// the 64 lanes have a tile's 16 tokens between them) under one scale.
+template <int HEAD>
+struct Rows {
+    static constexpr int kUnit = HEAD == 64 ? 16 : 32;
+    static constexpr int kUnitWords = kUnit / 8;       // dwords of codes
+    static constexpr int kUnits = HEAD / kUnit;        // of a token: 4, 4, 6, 8
+    static constexpr int kPasses = (kUnits + 3) / 4;   // of 64 lanes over a tile
+    static constexpr int kChunks = HEAD / 8;           // 16-byte chunks of a row
+    static constexpr int kSwizzle = HEAD % 128 == 0 ? 16 : 8;
+    static constexpr int kCols = HEAD / 16;            // blocks of 16 columns
+    static constexpr int kGroups = HEAD / 32;          // scales of a row
+    // K: row-major, chunks swizzled by the row
+    static __device__ __forceinline__ int kSlot(int row, int chunk) { return row * kChunks + (chunk ^ (row & (kSwizzle - 1))); }
+    // V: [row half (8 rows)][block of 16 columns][row of the half][two chunks, exchanged in the upper half], so that neither
+    // the transposing reads nor the writes of 16 tokens meet in a bank
+    static __device__ __forceinline__ int vSlot(int row, int chunk) {
+        return (row >> 3) * 8 * kChunks + (chunk >> 1) * 16 + (row & 7) * 2 + ((chunk & 1) ^ (row >> 3));
+    }
+};
+
+// Tokens per step: 64, but 32 at head 192 with 64 rows, where two workgroups then share a compute unit's LDS.
+template <int HEAD, int R>
+constexpr int stepTokens() { return HEAD == 192 && R == 1 ? 32 : 64; }
+template <int HEAD, int R>
+constexpr int workgroupsPerUnit() { return HEAD <= 128 || (HEAD == 192 && R == 1) ? 2 : 1; }
+
+// WHOLE: the page size is a multiple of 16, so that a tile lies in one page; otherwise every lane looks its rows up.
+template <typename T, int HEAD, int R, bool WHOLE>
+__global__ void __launch_bounds__(kPrefillThreads, (workgroupsPerUnit<HEAD, R>())) prefillFp4Kernel(PrefillFp4Args a) {
+    using S = typename T::storage;
+    using G = Rows<HEAD>;
+    constexpr int BM = 64 * R, BN = stepTokens<HEAD, R>(), TT = BN / kTile;
+    constexpr int kTileSlots = kTile * G::kChunks;
+    struct Tiles {
+        uint4 k[2][TT * kTileSlots], v[2][TT * kTileSlots];
+    };
+    __shared__ Tiles tiles;
+    // values that are not finite: bit t of [step % 3][scale group] = token t of the step
+    __shared__ unsigned long long bad[3][G::kGroups];
+    __shared__ int any_bad[3];
+
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kv_head = blockIdx.x % a.num_kv_heads;
+
+    int seq, block;
+    Span span;
+    if (!findBlock(a, lane, BM, blockIdx.x / a.num_kv_heads, seq, block, span)) {
+        return;
+    }
+    const int total_rows = span.q_len * a.group;
+    const int block_row0 = block * BM;
+    const int last_row = min(block_row0 + BM, total_rows) - 1;
+    const int block_visible = __builtin_amdgcn_readfirstlane(visibleTokens(a, span, last_row / a.group));
+    if (block_visible <= 0) {
+        return;
+    }
+    const int n_steps = (block_visible + BN - 1) / BN;
+
+    if (threadIdx.x < 3 * G::kGroups) {
+        (&bad[0][0])[threadIdx.x] = 0;
+    }
+    if (threadIdx.x < 3) {
+        any_bad[threadIdx.x] = 0;
+    }
+
+    // ---- this lane's columns: row c of each of the wavefront's R groups of 16 rows ----
+    uint4 q_reg[R][HEAD / 32];
+    int visible[R];
+    float slope[R];
+    int most_visible = 0, least_visible = 0x7fffffff;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int row = block_row0 + (w * R + r) * 16 + c;
+        const bool valid = row < total_rows;
+        const int token = valid ? row / a.group : 0;
+        const int head = kv_head * a.group + (valid ? row - token * a.group : 0);
+        visible[r] = valid ? visibleTokens(a, span, token) : 0;
+        slope[r] = a.alibi_slopes != nullptr && valid ? a.alibi_slopes[head] * kLog2e : 0.0f;
+        const S *from = static_cast<const S *>(a.q) + (span.q_start + token) * a.q_stride + head * a.q_head_stride;
+#pragma unroll
+        for (int kk = 0; kk < HEAD / 32; ++kk) {
+            const S *at = from + 32 * kk + 8 * g;
+            uint4 x;
+            if (a.q_aligned) {
+                x = *reinterpret_cast<const uint4 *>(at);
+            } else {
+                const uint16_t *e = reinterpret_cast<const uint16_t *>(at);
+                x = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+            }
+            q_reg[r][kk] = valid ? x : make_uint4(0, 0, 0, 0);
+        }
+        most_visible = max(most_visible, visible[r]);
+        least_visible = min(least_visible, valid ? visible[r] : 0x7fffffff);
+    }
+    most_visible = __builtin_amdgcn_readfirstlane(waveMaxInt(most_visible));
+    least_visible = __builtin_amdgcn_readfirstlane(-waveMaxInt(-least_visible));
+
+    // ---- loads: codes and scales of this wavefront's tile of a step (TT = 4: tile w of K and V; TT = 2: wavefronts 0, 1 take
+    // the tiles of K, 2, 3 those of V) ----
+    const bool loads_k = TT == 4 || w < 2, loads_v = TT == 4 || w >= 2;
+    const int own_tile = TT == 4 ? w : (w & 1);
+    const int64_t table_row = seq * a.block_table_stride;
+    const int last_entry = (block_visible - 1) / a.block_size;
+    auto entryId = [&](int entry) { return clampPage(loadIndexOf(a.index_type, a.block_tables, table_row + min(entry, last_entry)), a.num_blocks); };
+
+    struct Raw { // what a lane has loaded, per pass
+        uint32_t k[G::kPasses][G::kUnitWords], v[G::kPasses][G::kUnitWords];
+        uint32_t ks[G::kPasses], vs[G::kPasses];
+    };
+    Raw raw;
+    // which row of the tile and which unit of it this lane has: K unit-fastest (contiguous loads), V token-fastest (see vSlot)
+    auto kRow = [&](int p) { return (64 * p + lane) / G::kUnits; };
+    auto kUnitOf = [&](int p) { return (64 * p + lane) % G::kUnits; };
+    auto vRow = [&](int p) { return lane & 15; };
+    auto vUnitOf = [&](int p) { return (64 * p + lane) >> 4; };
+    auto has = [&](int p) { return 64 * p + lane < kTile * G::kUnits; };
+
+    // table entries of 64 pages, a batch ahead (WHOLE)
+    int batch = 0, ids = 0, ids_next = 0;
+    int entry = kTile * own_tile / a.block_size, row_in_page = kTile * own_tile - entry * a.block_size; // of the tile that comes next
+    if constexpr (WHOLE) {
+        ids = entryId(lane);
+        ids_next = entryId(64 + lane);
+    }
+    auto load = [&](int step) {
+        const int t = step * BN + kTile * own_tile;
+        if constexpr (WHOLE) {
+            if (t < block_visible) {
+                while (row_in_page >= a.block_size) {
+                    row_in_page -= a.block_size;
+                    ++entry;
+                }
+            } else { // behind what the block sees: the last tile that it does, again
+                entry = last_entry;
+                row_in_page = (block_visible - 1) / kTile * kTile - entry * a.block_size;
+            }
+            const int e = entry, row0 = row_in_page;
+            row_in_page += BN;
+            if ((e >> 6) > batch) {
+                ++batch;
+                ids = ids_next;
+                ids_next = entryId(64 * (batch + 1) + lane);
+            }
+            const int64_t id = __builtin_amdgcn_readlane(ids, e & 63);
+            auto tile = [&](const PoolSide &s) { return s.base + id * s.block + kv_head * s.head + static_cast<int64_t>(row0) * s.row; };
+            if (loads_k) {
+                const char *codes = tile(a.k_codes), *scales = tile(a.k_scales);
+#pragma unroll
+                for (int p = 0; p < G::kPasses; ++p) {
+                    if (has(p)) {
+                        loadWords<4 * G::kUnitWords, false>(codes + kRow(p) * a.k_codes.row + kUnitOf(p) * (G::kUnit / 2), raw.k[p]);
+                        raw.ks[p] = static_cast<uint8_t>(scales[kRow(p) * a.k_scales.row + kUnitOf(p) * G::kUnit / 32]);
+                    }
+                }
+            }
+            if (loads_v) {
+                const char *codes = tile(a.v_codes), *scales = tile(a.v_scales);
+#pragma unroll
+                for (int p = 0; p < G::kPasses; ++p) {
+                    if (has(p)) {
+                        loadWords<4 * G::kUnitWords, false>(codes + vRow(p) * a.v_codes.row + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
+                        raw.vs[p] = static_cast<uint8_t>(scales[vRow(p) * a.v_scales.row + vUnitOf(p) * G::kUnit / 32]);
+                    }
+                }
+            }
+        } else {
+            auto rowOf = [&](const PoolSide &s, int64_t id, int row) { return s.base + id * s.block + kv_head * s.head + static_cast<int64_t>(row) * s.row; };
+#pragma unroll
+            for (int p = 0; p < G::kPasses; ++p) {
+                if (has(p)) {
+                    if (loads_k) {
+                        const int token = min(t + kRow(p), block_visible - 1), e = token / a.block_size;
+                        const int id = entryId(e), row = token - e * a.block_size;
+                        loadWords<4 * G::kUnitWords, false>(rowOf(a.k_codes, id, row) + kUnitOf(p) * (G::kUnit / 2), raw.k[p]);
+                        raw.ks[p] = static_cast<uint8_t>(rowOf(a.k_scales, id, row)[kUnitOf(p) * G::kUnit / 32]);
+                    }
+                    if (loads_v) {
+                        const int token = min(t + vRow(p), block_visible - 1), e = token / a.block_size;
+                        const int id = entryId(e), row = token - e * a.block_size;
+                        loadWords<4 * G::kUnitWords, false>(rowOf(a.v_codes, id, row) + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
+                        raw.vs[p] = static_cast<uint8_t>(rowOf(a.v_scales, id, row)[vUnitOf(p) * G::kUnit / 32]);
+                    }
+                }
+            }
+        }
+    };
+    // What was loaded for `step`, as 16-bit values in LDS. Rows that nobody of the block sees (behind the sequence's end, or
+    // behind the block's last row) may hold anything: their scores are masked, their values go in as zeros.
+    auto convert = [&](int step) {
+        if (loads_k) {
+            uint4 *to = tiles.k[step & 1] + own_tile * kTileSlots;
+#pragma unroll
+            for (int p = 0; p < G::kPasses; ++p) {
+                if (has(p)) {
+#pragma unroll
+                    for (int i = 0; i < G::kUnitWords; ++i) {
+                        to[G::kSlot(kRow(p), G::kUnitWords * kUnitOf(p) + i)] = toQueryType<T>(raw.k[p][i], mx::scaleOf(raw.ks[p]));
+                    }
+                }
+            }
+        }
+        if (loads_v) {
+            uint4 *to = tiles.v[step & 1] + own_tile * kTileSlots;
+            const int t = kTile * own_tile;
+#pragma unroll
+            for (int p = 0; p < G::kPasses; ++p) {
+                if (has(p)) {
+                    const bool seen = step * BN + t + vRow(p) < block_visible;
+                    const bool finite = raw.vs[p] != 0xff;
+                    const float scale = seen && finite ? mx::scaleOf(raw.vs[p]) : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < G::kUnitWords; ++i) {
+                        to[G::vSlot(vRow(p), G::kUnitWords * vUnitOf(p) + i)] = mx::toF16x8(raw.v[p][i], scale);
+                    }
+                    if (seen && !finite) {
+                        atomicOr(&bad[step % 3][vUnitOf(p) * G::kUnit / 32], 1ull << (t + vRow(p)));
+                        any_bad[step % 3] = 1;
+                    }
+                }
+            }
+        }
+    };
+
+    // ---- softmax state: o[r][e][i] = O[row c of group r][column 16 e + 4 g + i], ol[r] the row's denominator, m[r] its
+    // reference point in units of the raw product (of the score in log2 units with ALiBi or a scale that is not positive) ----
+    f32x4 o[R][G::kCols], ol[R];
+    float m[R], shift[R]; // shift: -m in log2 units, 0 while m = -inf
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int e = 0; e < G::kCols; ++e) {
+            o[r][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+        ol[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m[r] = -INFINITY;
+        shift[r] = 0.0f;
+    }
+    const bool plain = a.alibi_slopes == nullptr && a.scale_log2 > 0.0f;
+    const float unit = plain ? a.scale_log2 : 1.0f;
+    const float lazy = kLazyLog2 / unit;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 *LdsPiece;
+    // this lane's piece of a transposing read: token 4 g + c / 4 of the tile, columns 4 (c % 4) .. + 3 of the block
+    const auto v_read = (__attribute__((address_space(3))) char *)&tiles.v[0][0]
+                      + 16 * ((g >> 1) * 8 * G::kChunks + (4 * (g & 1) + (c >> 2)) * 2 + (((c & 3) >> 1) ^ (g >> 1))) + 8 * (c & 1);
+    const uint32_t one2 = TileF16::pack2(1.0f, 1.0f);
+    const uint4 ones = make_uint4(one2, one2, one2, one2);
+
+    auto compute = [&](int step, auto between) {
+        const int buf = step & 1, t0 = step * BN;
+        f32x4 s[R][TT];
+#pragma unroll
+        for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                s[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+#pragma unroll
+            for (int kk = 0; kk < HEAD / 32; ++kk) {
+                const uint4 k = tiles.k[buf][tt * kTileSlots + G::kSlot(c, 4 * kk + g)];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    s[r][tt] = T::mfmaK32(k, q_reg[r][kk], s[r][tt]);
+                }
+            }
+        }
+        between();
+        uint4 p_op[R][TT / 2];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (!plain) {
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[r][tt][i] = s[r][tt][i] * a.scale_log2 + slope[r] * static_cast<float>(t0 + 16 * tt + 4 * g + i - (visible[r] - 1));
+                    }
+                }
+            }
+            if (t0 + BN > least_visible) {
+#pragma unroll
+                for (int tt = 0; tt < TT; ++tt) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        s[r][tt][i] = t0 + 16 * tt + 4 * g + i >= visible[r] ? -INFINITY : s[r][tt][i];
+                    }
+                }
+            }
+            float top = maxOf(s[r][0][0], s[r][0][1]); // (three-operand maxima)
+#pragma unroll
+            for (int j = 2; j < 4 * TT; j += 2) {
+                top = maxOf(maxOf(top, s[r][j / 4][j % 4]), s[r][j / 4][j % 4 + 1]);
+            }
+            // (a row that has seen nothing has m = -inf: any finite maximum is above it; a NaN is above nothing, and reaches
+            // the outputs by its own probability)
+            if (__builtin_amdgcn_ballot_w64(top > m[r] + lazy) != 0) {
+                const float m_new = maxOf(m[r], maxAcrossTokenGroups(top));
+                const float alpha = m_new > m[r] ? fastExp2((m[r] - m_new) * unit) : 1.0f;
+                m[r] = m_new;
+                shift[r] = m_new == -INFINITY ? 0.0f : -m_new * unit;
+                ol[r] *= alpha;
+#pragma unroll
+                for (int e = 0; e < G::kCols; ++e) {
+                    o[r][e] *= alpha;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < TT / 2; ++u) {
+                uint32_t words[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4 x = s[r][2 * u + h];
+                    words[2 * h] = TileF16::pack2(fastExp2(__builtin_fmaf(x[0], unit, shift[r])), fastExp2(__builtin_fmaf(x[1], unit, shift[r])));
+                    words[2 * h + 1] = TileF16::pack2(fastExp2(__builtin_fmaf(x[2], unit, shift[r])), fastExp2(__builtin_fmaf(x[3], unit, shift[r])));
+                }
+                p_op[r][u] = make_uint4(words[0], words[1], words[2], words[3]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < TT / 2; ++u) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                ol[r] = TileF16::mfmaK32(ones, p_op[r][u], ol[r]);
+            }
+#pragma unroll
+            for (int e = 0; e < G::kCols; ++e) {
+                const auto at = v_read + (buf * TT + 2 * u) * (kTileSlots * 16) + 256 * e;
+                const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPiece>(at)));
+                const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsPiece>(at + kTileSlots * 16)));
+                const uint4 v = make_uint4(lo.x, lo.y, hi.x, hi.y);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    o[r][e] = TileF16::mfmaK32(v, p_op[r][u], o[r][e]);
+                }
+            }
+        }
+        if (any_bad[step % 3] != 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int n = visible[r] - t0;
+                const unsigned long long sees = n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1);
+#pragma unroll
+                for (int e = 0; e < G::kCols; ++e) {
+                    if ((bad[step % 3][e / 2] & sees) != 0) {
+                        o[r][e] = f32x4{NAN, NAN, NAN, NAN};
+                    }
+                }
+            }
+        }
+    };
+
+    // ---- pipeline: codes two steps ahead in registers, values one step ahead in LDS ----
+    load(0);
+    __syncthreads(); // the notes of values that are not finite are clear
+    convert(0);
+    if (n_steps > 1) {
+        load(1);
+    }
+    __syncthreads();
+    for (int step = 0; step < n_steps; ++step) {
+        if (threadIdx.x < G::kGroups) { // of step - 1, read before the last barrier, for step + 2
+            bad[(step + 2) % 3][threadIdx.x] = 0;
+            any_bad[(step + 2) % 3] = 0;
+        }
+        auto next = [&]() {
+            if (step + 1 < n_steps) {
+                convert(step + 1);
+                if (step + 2 < n_steps) {
+                    load(step + 2);
+                }
+            }
+        };
+        if (step * BN < most_visible) {
+            compute(step, next);
+        } else { // nothing that this wavefront's rows see
+            next();
+        }
+        __syncthreads();
+    }
+
+    // ---- normalise and store: a lane holds four consecutive columns of row c of a group; the wavefront's rows pass through
+    // LDS (nobody reads the tiles any more) and leave as 16-byte pieces ----
+    static_assert(sizeof(Tiles) >= 4 * R * 16 * HEAD * 2, "the tiles hold the output rows of all four wavefronts");
+    auto piece = [](int row, int chunk) { return row * G::kChunks + (chunk ^ (row & (G::kSwizzle - 1))); };
+    uint4 *stage = reinterpret_cast<uint4 *>(&tiles) + w * (R * 16 * G::kChunks);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const float f = 1.0f / ol[r][0];
+#pragma unroll
+        for (int e = 0; e < G::kCols; ++e) {
+            const f32x4 x = o[r][e];
+            reinterpret_cast<uint2 *>(stage + piece(r * 16 + c, 2 * e + (g >> 1)))[g & 1] =
+                make_uint2(T::pack2(x[0] * f, x[1] * f), T::pack2(x[2] * f, x[3] * f));
+        }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the wavefront's own stores, before its lanes read one another's
+#pragma unroll
+    for (int i = 0; i < R * 16 * G::kChunks / 64; ++i) {
+        const int at = 64 * i + lane;
+        const int local = at / G::kChunks, chunk = at % G::kChunks;
+        const int row = block_row0 + w * R * 16 + local;
+        if (row >= total_rows) {
+            continue;
+        }
+        const int token = row / a.group;
+        if (visibleTokens(a, span, token) <= 0) {
+            continue;
+        }
+        const int head = kv_head * a.group + (row - token * a.group);
+        const uint4 x = stage[piece(local, chunk)];
+        S *to = static_cast<S *>(a.out) + (span.q_start + token) * a.o_stride + head * a.o_head_stride + 8 * chunk;
+        if (a.out_aligned) {
+            *reinterpret_cast<uint4 *>(to) = x;
+        } else {
+            const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                reinterpret_cast<uint16_t *>(to)[j] = static_cast<uint16_t>(words[j / 2] >> (16 * (j & 1)));
+            }
+        }
+    }
+}
+
+} // namespace op::paged_attention_prefill_fp4::amd
+
+#endif

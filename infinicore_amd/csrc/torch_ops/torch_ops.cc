@@ -60,6 +60,7 @@ constexpr Operator kOperators[] = {
     {7, 2, 2, false, false, 2, true},    // paged_reading_fp4: k, v, k_codes, v_codes, k_scales, v_scales, slot_mapping
     {9, 1, 1, true, false, 2, true},     // paged_attention_fp4: out, q, k_codes, v_codes, k_scales, v_scales, block_tables,
                                          // cache_lens, alibi_slopes
+    {10, 1, 1, true, false, 2, true},    // paged_attention_prefill_fp4: ... block_tables, seq_lens, cum_seq_lens_q, alibi_slopes
 };
 constexpr int kNumOperators = sizeof(kOperators) / sizeof(kOperators[0]);
 constexpr int kMaxTensors = 10;
@@ -145,6 +146,7 @@ int callLibrary(int kind, const Entry &e, void *workspace, void *const *p, void 
     case 6: return reinterpret_cast<int (*)(V, V, size_t, V, V, V, V, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], stream);
     case 7: return reinterpret_cast<int (*)(V, V, size_t, V, V, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], stream);
     case 8: return reinterpret_cast<int (*)(V, V, size_t, V, C, C, C, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], stream);
+    case 9: return reinterpret_cast<int (*)(V, V, size_t, V, C, C, C, C, C, C, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], stream);
     default: return reinterpret_cast<int (*)(V, V, size_t, V, V, C, C, C, V)>(fn)(e.descriptor, workspace, e.workspace_bytes, p[0], p[1], p[2], p[3], p[4], stream);
     }
 }

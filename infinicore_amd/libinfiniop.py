@@ -197,6 +197,10 @@ def _open():
     _declare(op, "infiniopGetPagedAttentionFp4WorkspaceSize", [D, POINTER(c_size_t)])
     _declare(op, "infiniopPagedAttentionFp4", [D, vp, c_size_t] + [vp] * 10)
     _declare(op, "infiniopDestroyPagedAttentionFp4Descriptor", [D])
+    _declare(op, "infiniopCreatePagedAttentionPrefillFp4Descriptor", [infiniopHandle_t, POINTER(D)] + [T] * 10 + [c_float])
+    _declare(op, "infiniopGetPagedAttentionPrefillFp4WorkspaceSize", [D, POINTER(c_size_t)])
+    _declare(op, "infiniopPagedAttentionPrefillFp4", [D, vp, c_size_t] + [vp] * 11)
+    _declare(op, "infiniopDestroyPagedAttentionPrefillFp4Descriptor", [D])
     return rt, op
 
 

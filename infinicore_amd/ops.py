@@ -57,10 +57,10 @@ def _load_native():
 _native = _load_native()
 # the operators by number, as csrc/torch_ops/torch_ops.cc lists them
 (_PAGED_ATTENTION, _PAGED_ATTENTION_PREFILL, _PAGED_CACHING, _ROPE_PAGED_CACHING, _ROPE_QK_PAGED_CACHING, _KV_CACHING,
- _PAGED_CACHING_FP4, _PAGED_READING_FP4, _PAGED_ATTENTION_FP4) = range(9)
+ _PAGED_CACHING_FP4, _PAGED_READING_FP4, _PAGED_ATTENTION_FP4, _PAGED_ATTENTION_PREFILL_FP4) = range(10)
 _RUN = ("infiniopPagedAttention", "infiniopPagedAttentionPrefill", "infiniopPagedCaching", "infiniopRoPEPagedCaching",
         "infiniopRoPEQKPagedCaching", "infiniopKVCaching", "infiniopPagedCachingFp4", "infiniopPagedReadingFp4",
-        "infiniopPagedAttentionFp4")
+        "infiniopPagedAttentionFp4", "infiniopPagedAttentionPrefillFp4")
 _native.setup(tuple(ctypes.cast(getattr(LIBINFINIOP, name), c_void_p).value for name in _RUN),
               ctypes.cast(lib.LIBINFINIRT.infinirtSetDevice, c_void_p).value, int(InfiniDevice.AMD), _PLAN_CACHE_CAPACITY)
 
@@ -163,6 +163,12 @@ def _make_paged_attention_fp4(scale, *tensors):
                  "infiniopDestroyPagedAttentionFp4Descriptor", tensors[1].device, tensors[:-1], scale, optional=tensors[-1:])
 
 
+def _make_paged_attention_prefill_fp4(scale, *tensors):
+    return _plan("infiniopCreatePagedAttentionPrefillFp4Descriptor", "infiniopGetPagedAttentionPrefillFp4WorkspaceSize",
+                 "infiniopDestroyPagedAttentionPrefillFp4Descriptor", tensors[1].device, tensors[:-1], scale,
+                 optional=tensors[-1:])
+
+
 def _call(operator, number, make, *tensors):
     result = _native.call(operator, number, make, *tensors)
     if type(result) is int:  # a status; otherwise the output, both outputs or the first tensor
@@ -259,3 +265,12 @@ def paged_attention_fp4(q, k_codes, v_codes, k_scales, v_scales, block_tables, c
     ``paged_attention``: heads of 64, 128, 192 or 256, keys and values of one size."""
     return _call(_PAGED_ATTENTION_FP4, scale, _make_paged_attention_fp4, out, q, k_codes, v_codes, k_scales, v_scales,
                  block_tables, cache_lens, alibi_slopes)
+
+
+def paged_attention_prefill_fp4(q, k_codes, v_codes, k_scales, v_scales, block_tables, seq_lens, cum_seq_lens_q,
+                                alibi_slopes=None, scale: float = 1.0, *, out=None):
+    """Causal attention of each sequence's run of new tokens over its K/V in a pool held in 4 bits, the new tokens' own among
+    them; returns ``out``. The 4-bit counterpart of ``paged_attention_prefill``: heads of 64, 128, 192 or 256, keys and
+    values of one size."""
+    return _call(_PAGED_ATTENTION_PREFILL_FP4, scale, _make_paged_attention_prefill_fp4, out, q, k_codes, v_codes, k_scales,
+                 v_scales, block_tables, seq_lens, cum_seq_lens_q, alibi_slopes)

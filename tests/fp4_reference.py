@@ -1,5 +1,5 @@
 """The pool held in 4 bits and attention over it, in 64 bits from the definitions (include/infiniop/ops/paged_caching_fp4.h).
-Host tensors in, float64 out; nothing of the package is used."""
+Tensors of any device in, float64 out; nothing of the package is used."""
 from __future__ import annotations
 
 import math
@@ -7,6 +7,8 @@ import math
 import torch
 
 GROUP = 32
+NAN_BYTE = 255
+DEVICE = "cuda:0"  # of make_batch
 MAGNITUDES = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64)
 
 
@@ -101,3 +103,42 @@ def make_pool(seed, blocks, heads, page, size, *, spread=1.0):
         channel = torch.exp(spread * torch.randn((heads, 1, size), generator=gen))
         made.append(quantise(torch.randn((blocks, heads, page, size), generator=gen) * channel))
     return made[0][0], made[1][0], made[0][1], made[1][1]
+
+
+def make_batch(seed, lens, heads, kv_heads, d, page, dtype, *, index=torch.int64, layout="packed", spare=3, poison=True, hot=None, rows=None):
+    """A pool on the device, with the pages of `lens` in any order; every row that no sequence holds reads as NaN, table
+    entries behind a sequence's pages name pages that do not exist."""
+    gen = torch.Generator().manual_seed(seed)
+    needed = [max(0, -(-n // page)) for n in lens]
+    blocks = sum(needed) + spare
+    pool = make_pool(seed + 1, blocks, kv_heads, page, d)
+    pages = torch.randperm(blocks, generator=gen)
+    width = max([1, *needed]) + 2
+    table = torch.full((len(lens), width), 1 << 30, dtype=torch.int64)
+    table[:, 1::2] = -7
+    held = torch.zeros((blocks, page), dtype=torch.bool)
+    at = 0
+    for i, (n, count) in enumerate(zip(lens, needed)):
+        table[i, :count] = pages[at:at + count]
+        if count:
+            flat = held[pages[at:at + count]].flatten()
+            flat[:n] = True
+            held[pages[at:at + count]] = flat.view(count, page)
+        at += count
+    if index == torch.uint32:
+        table = table.clamp(min=0)
+    if poison:
+        away = ~held[:, None, :, None]
+        pool = [torch.where(away, 0x77 if t.shape[-1] == d // 2 else NAN_BYTE, t).to(torch.uint8) for t in pool]
+    pool = [t.to(DEVICE) for t in pool]
+    if layout == "rows":  # pages stored [rows, heads]
+        pool = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in pool]
+    elif layout == "padded":
+        wide = [torch.zeros((blocks + 1, kv_heads + 1, page + 1, 16 * -(-t.shape[-1] // 16) + 16), dtype=torch.uint8, device=DEVICE) for t in pool]
+        pool = [w[1:, 1:, 1:, :t.shape[-1]].copy_(t) for w, t in zip(wide, pool)]
+    q = torch.randn((len(lens) if rows is None else rows, heads, d), generator=gen)
+    if hot is not None:
+        q = q * hot
+    return dict(q=q.to(dtype).to(DEVICE), pool=pool, table=table.to(index).to(DEVICE), lens=torch.tensor(lens, dtype=index, device=DEVICE)
+                if index != torch.uint32 else torch.tensor([max(n, 0) for n in lens]).to(index).to(DEVICE),
+                needed=needed, scale=1 / math.sqrt(d))

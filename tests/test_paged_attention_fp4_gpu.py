@@ -13,46 +13,7 @@ from infinicore_amd import ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
-NAN_BYTE = 255
-
-
-def make_batch(seed, lens, heads, kv_heads, d, page, dtype, *, index=torch.int64, layout="packed", spare=3, poison=True, hot=None):
-    """A pool on the device, with the pages of `lens` in any order; every row that no sequence holds reads as NaN, table
-    entries behind a sequence's pages name pages that do not exist."""
-    gen = torch.Generator().manual_seed(seed)
-    needed = [max(0, -(-n // page)) for n in lens]
-    blocks = sum(needed) + spare
-    pool = fp4.make_pool(seed + 1, blocks, kv_heads, page, d)
-    pages = torch.randperm(blocks, generator=gen)
-    width = max([1, *needed]) + 2
-    table = torch.full((len(lens), width), 1 << 30, dtype=torch.int64)
-    table[:, 1::2] = -7
-    held = torch.zeros((blocks, page), dtype=torch.bool)
-    at = 0
-    for i, (n, count) in enumerate(zip(lens, needed)):
-        table[i, :count] = pages[at:at + count]
-        if count:
-            flat = held[pages[at:at + count]].flatten()
-            flat[:n] = True
-            held[pages[at:at + count]] = flat.view(count, page)
-        at += count
-    if index == torch.uint32:
-        table = table.clamp(min=0)
-    if poison:
-        away = ~held[:, None, :, None]
-        pool = [torch.where(away, 0x77 if t.shape[-1] == d // 2 else NAN_BYTE, t).to(torch.uint8) for t in pool]
-    pool = [t.to(DEV) for t in pool]
-    if layout == "rows":  # pages stored [rows, heads]
-        pool = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in pool]
-    elif layout == "padded":
-        wide = [torch.zeros((blocks + 1, kv_heads + 1, page + 1, 16 * -(-t.shape[-1] // 16) + 16), dtype=torch.uint8, device=DEV) for t in pool]
-        pool = [w[1:, 1:, 1:, :t.shape[-1]].copy_(t) for w, t in zip(wide, pool)]
-    q = torch.randn((len(lens), heads, d), generator=gen)
-    if hot is not None:
-        q = q * hot
-    return dict(q=q.to(dtype).to(DEV), pool=pool, table=table.to(index).to(DEV), lens=torch.tensor(lens, dtype=index, device=DEV)
-                if index != torch.uint32 else torch.tensor([max(n, 0) for n in lens]).to(index).to(DEV),
-                needed=needed, scale=1 / math.sqrt(d))
+NAN_BYTE = fp4.NAN_BYTE
 
 
 def reference(b, lens, slopes=None, scale=None):
@@ -96,7 +57,7 @@ BORDERS = [0, 1, 2, 15, 16, 17, 31, 32, 33, 47, 63, 64, 65, 127, 129, -3, 500, 7
 @pytest.mark.parametrize("page", [16, 32, 8, 24, 1, 7, 48])
 def test_lengths_sizes_pages(dtype, d, page):
     print("case", dtype, d, page, flush=True)
-    check(make_batch(d + page, BORDERS, 8, 2, d, page, dtype), BORDERS)
+    check(fp4.make_batch(d + page, BORDERS, 8, 2, d, page, dtype), BORDERS)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -104,20 +65,20 @@ def test_lengths_sizes_pages(dtype, d, page):
 def test_head_layouts(dtype, heads, kv_heads):
     print("case", dtype, heads, kv_heads, flush=True)
     lens = [1, 70, 333, 0, 1025]
-    check(make_batch(heads, lens, heads, kv_heads, 128, 16, dtype), lens)
+    check(fp4.make_batch(heads, lens, heads, kv_heads, 128, 16, dtype), lens)
 
 
 @pytest.mark.parametrize("index", [torch.int64, torch.int32, torch.uint32])
 @pytest.mark.parametrize("layout", ["packed", "rows", "padded"])
 def test_indices_and_layouts(index, layout):
     lens = [5, 0, 200, 64, 1]
-    check(make_batch(3, lens, 16, 4, 128, 16, torch.bfloat16, index=index, layout=layout), lens)
+    check(fp4.make_batch(3, lens, 16, 4, 128, 16, torch.bfloat16, index=index, layout=layout), lens)
 
 
 @pytest.mark.parametrize("d,page", [(64, 16), (128, 8), (192, 16), (256, 5)])
 def test_query_and_output_strides(d, page):
     lens = [40, 3, 0, 130]
-    b = make_batch(9, lens, 12, 4, d, page, torch.float16)
+    b = fp4.make_batch(9, lens, 12, 4, d, page, torch.float16)
     fused = torch.zeros((4, 20, d), dtype=torch.float16, device=DEV)  # q as a slice of a projection
     fused[:, 3:15] = b["q"]
     odd = torch.zeros((4, 12, d + 1), dtype=torch.float16, device=DEV)
@@ -135,31 +96,31 @@ def test_query_and_output_strides(d, page):
 def test_alibi(dtype, d):
     lens = [1, 100, 0, 1531, 64]
     slopes = torch.tensor([2.0 ** (-8 * (h + 1) / 16) for h in range(16)], device=DEV)
-    check(make_batch(4, lens, 16, 16, d, 32, dtype, index=torch.int32), lens, slopes)
+    check(fp4.make_batch(4, lens, 16, 16, d, 32, dtype, index=torch.int32), lens, slopes)
     slopes = torch.cat((-slopes[:6], torch.zeros(6, device=DEV)))  # rising with the distance, and none
-    check(make_batch(5, lens, 10, 2, d, 16, dtype), lens, slopes)
+    check(fp4.make_batch(5, lens, 10, 2, d, 16, dtype), lens, slopes)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.125, 1.0])
 def test_scales(scale):
     lens = [1, 90, 300]
-    check(make_batch(6, lens, 8, 2, 128, 16, torch.bfloat16), lens, scale=scale)
+    check(fp4.make_batch(6, lens, 8, 2, 128, 16, torch.bfloat16), lens, scale=scale)
 
 
 @pytest.mark.parametrize("page", [16, 7])
 def test_one_long_sequence_and_many_short(page):
-    check(make_batch(7, [40001], 16, 2, 128, page, torch.bfloat16), [40001])
+    check(fp4.make_batch(7, [40001], 16, 2, 128, page, torch.bfloat16), [40001])
     lens = [(37 * i) % 90 for i in range(333)]
-    check(make_batch(8, lens, 8, 2, 64, page, torch.float16), lens)
+    check(fp4.make_batch(8, lens, 8, 2, 64, page, torch.float16), lens)
     lens = [3, 9000, 1, 0, 5000, 2]
-    check(make_batch(8, lens, 32, 8, 128, page, torch.float16), lens)
+    check(fp4.make_batch(8, lens, 32, 8, 128, page, torch.float16), lens)
 
 
 def test_climbing_scores():
     """The maximum moves in every tile, below and above the threshold for moving the reference point."""
     lens = [900, 2100]
     for hot in (1.0, 30.0, 300.0):
-        b = make_batch(10, lens, 8, 2, 128, 16, torch.bfloat16, hot=hot)
+        b = fp4.make_batch(10, lens, 8, 2, 128, 16, torch.bfloat16, hot=hot)
         for i, n in enumerate(lens):  # later rows hold larger keys along the query
             pages = b["table"][i, :b["needed"][i]].long()
             order = torch.arange(len(pages) * 16, device=DEV).view(-1, 1, 16, 1)
@@ -170,7 +131,7 @@ def test_climbing_scores():
 
 def test_a_visible_nan_stays_in_its_sequence_and_head():
     lens = [70, 300, 129]
-    b = make_batch(11, lens, 8, 2, 128, 16, torch.bfloat16)
+    b = fp4.make_batch(11, lens, 8, 2, 128, 16, torch.bfloat16)
     clean = check(b, lens)
     page = int(b["table"][1, 17])
     b["pool"][2][page, 1, 5, 2] = NAN_BYTE  # a key of sequence 1, KV head 1
@@ -189,7 +150,7 @@ def test_a_visible_nan_stays_in_its_sequence_and_head():
 def test_products_that_overflow():
     """Queries so large that products with keys are infinite in 32 bits: -inf has no weight, +inf and NaN reach the output."""
     lens = [100]
-    b = make_batch(12, lens, 1, 1, 64, 16, torch.bfloat16)
+    b = fp4.make_batch(12, lens, 1, 1, 64, 16, torch.bfloat16)
     codes = torch.zeros_like(b["pool"][0])
     codes[..., 0] = 0x0F  # -6 in the first element of every key
     pages = b["table"][0, :7].long()
@@ -206,7 +167,7 @@ def test_products_that_overflow():
 
 def test_page_order_repeats_and_lengths_beyond_the_table():
     lens = [333, 1000, 17]
-    b = make_batch(13, lens, 8, 2, 128, 16, torch.float16)
+    b = fp4.make_batch(13, lens, 8, 2, 128, 16, torch.float16)
     first = check(b, lens)
     assert torch.equal(check(b, lens), first)
     blocks = b["pool"][0].shape[0]
@@ -243,7 +204,7 @@ def test_offsets_past_32_bits():
 
 def test_streams_and_graphs():
     lens = [300, 40, 1200]
-    b = make_batch(14, lens, 32, 8, 128, 16, torch.bfloat16, poison=False)
+    b = fp4.make_batch(14, lens, 32, 8, 128, 16, torch.bfloat16, poison=False)
     args = (b["q"], *b["pool"], b["table"], b["lens"], None, b["scale"])
     eager = ops.paged_attention_fp4(*args)
     side = torch.cuda.Stream()
@@ -275,7 +236,7 @@ def test_streams_and_graphs():
 
 def test_c_entry_points():
     lens = [100, 2000]
-    b = make_batch(15, lens, 16, 4, 128, 16, torch.bfloat16)
+    b = fp4.make_batch(15, lens, 16, 4, 128, 16, torch.bfloat16)
     out = torch.full_like(b["q"], 7.0)
     tensors = [out, b["q"], *b["pool"], b["table"], b["lens"]]
     L.set_device(L.InfiniDevice.AMD, 0)
