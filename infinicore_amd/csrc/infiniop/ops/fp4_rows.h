@@ -1,0 +1,133 @@
+// What writing tokens into a 4-bit pool and reading them back have in common: which lane has which eight elements of which
+// token, and where they lie in the pool.
+#ifndef INFINICORE_AMD_FP4_ROWS_H
+#define INFINICORE_AMD_FP4_ROWS_H
+
+#include "fp4_pool.h"
+#include <cstdint>
+#include <hip/hip_runtime.h>
+
+namespace op::fp4 {
+
+constexpr int kRowThreads = 256;
+constexpr int kRowElements = 8; // of a lane; four lanes are a group under one scale
+
+// Keys or values: the pool's side (strides in bytes) and the side of 16- or 32-bit values (strides in elements).
+template <typename Byte, typename Void>
+struct RowSide {
+    Byte *codes, *scales;
+    Void *wide;
+    int64_t code_block, code_head, code_row;
+    int64_t scale_block, scale_head, scale_row;
+    int64_t token_stride, head_stride;
+    uint32_t lanes_per_row; // size / 8
+};
+
+template <typename Byte, typename Void>
+struct RowArgs {
+    RowSide<Byte, Void> k, v;
+    const int64_t *slot_mapping;
+    int64_t num_slots;
+    uint32_t num_tokens;
+    uint32_t k_lanes;      // of a token: heads x k.lanes_per_row
+    uint32_t token_lanes;  // of its keys and values
+    uint32_t token_groups; // tokens that a workgroup has at a time
+    uint32_t block_size;
+    int32_t block_shift;   // log2(block_size) when it is a power of two, else -1
+};
+
+// One lane's place in every token it works on.
+template <typename Byte, typename Void>
+struct RowLane {
+    bool exists;
+    uint32_t token; // of the first round; a round later it is token_groups further on
+    uint32_t head, chunk;
+    bool first_of_group; // the lane that has the scale byte
+    Byte *codes, *scales;
+    int64_t code_block, code_row, scale_block, scale_row;
+    int64_t token_stride;
+    int64_t in_token; // element offset in a token of the wide side
+    Void *wide;
+
+    // blockIdx.x: ROUNDS x token_groups tokens; blockIdx.y: 256 lanes of a token that has more
+    __device__ __forceinline__ RowLane(const RowArgs<Byte, Void> &a, uint32_t rounds) {
+        const uint32_t t = token_lanes(a) ? threadIdx.x / a.token_lanes : 0;
+        uint32_t u = threadIdx.x - t * a.token_lanes + blockIdx.y * kRowThreads;
+        exists = t < a.token_groups && u < a.token_lanes;
+        token = blockIdx.x * rounds * a.token_groups + t;
+        const bool value = u >= a.k_lanes;
+        u -= value ? a.k_lanes : 0;
+        const RowSide<Byte, Void> &s = value ? a.v : a.k;
+        head = u / s.lanes_per_row;
+        chunk = u - head * s.lanes_per_row;
+        first_of_group = (chunk & 3) == 0;
+        codes = s.codes + head * s.code_head + chunk * 4;
+        scales = s.scales + head * s.scale_head + (chunk >> 2);
+        code_block = s.code_block, code_row = s.code_row, scale_block = s.scale_block, scale_row = s.scale_row;
+        token_stride = s.token_stride;
+        in_token = head * s.head_stride + chunk * kRowElements;
+        wide = s.wide;
+    }
+    static __device__ __forceinline__ bool token_lanes(const RowArgs<Byte, Void> &a) { return a.token_lanes < kRowThreads; }
+    static __device__ __forceinline__ void place(const RowArgs<Byte, Void> &a, int64_t slot, int64_t &page, int64_t &row) {
+        page = a.block_shift >= 0 ? slot >> a.block_shift : slot / a.block_size;
+        row = slot - page * a.block_size;
+    }
+};
+
+// Rounds of tokens that a workgroup takes, all loads of a turn before its stores: more loads in flight and less arithmetic per
+// element, where a device of `units` compute units has enough workgroups all the same. us for 1 / 2 / 4 rounds, bf16, 8 heads
+// of 128: reading 65 536 tokens 138 / 78 / 73, 4 096 9.0 / 8.2 / 9.3; writing 4 096 8.1 / 7.1 / 7.0; 16 heads of 64, 1 531 tokens,
+// reading 5.4 / 6.1 with two, writing 5.4 / 5.2.
+inline int rowRounds(uint64_t workgroups, int units) {
+    return workgroups >= static_cast<uint64_t>(units) * 32 ? 4 : (workgroups >= static_cast<uint64_t>(units) * 12 ? 2 : 1);
+}
+
+template <typename Byte, typename Void>
+RowSide<Byte, Void> rowSide(Byte *codes, Byte *scales, Void *wide, const PoolStrides &c, const PoolStrides &s,
+                            ptrdiff_t token_stride, ptrdiff_t head_stride, size_t size) {
+    return {codes, scales, wide, c.block, c.head, c.row, s.block, s.head, s.row, token_stride, head_stride,
+            static_cast<uint32_t>(size / kRowElements)};
+}
+
+template <typename Byte, typename Void>
+struct RowLaunch {
+    RowArgs<Byte, Void> args;
+    bool aligned; // wide rows at multiples of 16 bytes, rows of codes at multiples of 4
+    int rounds;   // 1, 2 or 4
+    dim3 grid;
+};
+
+// Lanes, grid and alignment of a call; `wide_bytes`: of an element.
+template <typename Byte, typename Void, typename Info>
+RowLaunch<Byte, Void> rowLaunch(const Info &in, Byte *k_codes, Byte *v_codes, Byte *k_scales, Byte *v_scales, Void *k, Void *v,
+                                const void *slot_mapping, size_t wide_bytes, int units) {
+    const PoolInfo &pool = in.pool;
+    RowLaunch<Byte, Void> l{};
+    RowArgs<Byte, Void> &a = l.args;
+    a.k = rowSide(k_codes, k_scales, k, pool.k_codes, pool.k_scales, in.k_token_stride, in.k_head_stride, pool.k_size);
+    a.v = rowSide(v_codes, v_scales, v, pool.v_codes, pool.v_scales, in.v_token_stride, in.v_head_stride, pool.v_size);
+    a.slot_mapping = static_cast<const int64_t *>(slot_mapping);
+    a.num_slots = static_cast<int64_t>(pool.num_blocks) * static_cast<int64_t>(pool.block_size);
+    a.num_tokens = static_cast<uint32_t>(in.num_tokens);
+    a.k_lanes = static_cast<uint32_t>(pool.num_kv_heads) * a.k.lanes_per_row;
+    a.token_lanes = a.k_lanes + static_cast<uint32_t>(pool.num_kv_heads) * a.v.lanes_per_row;
+    a.token_groups = a.token_lanes >= kRowThreads ? 1 : kRowThreads / a.token_lanes;
+    a.block_size = static_cast<uint32_t>(pool.block_size);
+    a.block_shift = a.block_size > 0 && (a.block_size & (a.block_size - 1)) == 0 ? __builtin_ctz(a.block_size) : -1;
+
+    auto address = [](const void *p) { return reinterpret_cast<uint64_t>(p); };
+    const uint64_t strides = (in.num_tokens > 1 ? in.k_token_stride | in.v_token_stride : 0)
+                           | (pool.num_kv_heads > 1 ? in.k_head_stride | in.v_head_stride : 0);
+    l.aligned = (address(k) | address(v) | strides * wide_bytes) % 16 == 0 && (address(k_codes) | address(v_codes)) % 4 == 0
+             && pool.codeRowsAligned(4);
+    const uint32_t turns = (a.num_tokens + a.token_groups - 1) / a.token_groups;
+    const uint32_t y = (a.token_lanes + kRowThreads - 1) / kRowThreads;
+    l.rounds = l.aligned ? rowRounds(static_cast<uint64_t>(turns) * y, units) : 1;
+    l.grid = dim3((turns + l.rounds - 1) / l.rounds, y);
+    return l;
+}
+
+} // namespace op::fp4
+
+#endif

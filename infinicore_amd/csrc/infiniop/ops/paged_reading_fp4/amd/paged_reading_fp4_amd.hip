@@ -5,7 +5,9 @@
 #include "paged_reading_fp4_amd.h"
 #include "../../../devices/amd/amd_fp4.h"
 #include "../../../devices/amd/amd_streaming.h"
+#include "../../../devices/amd/amd_device.h"
 #include "../../../handle.h"
+#include "../../fp4_rows.h"
 #include "../../../../utils/check.h"
 
 namespace op::paged_reading_fp4::amd {
@@ -14,29 +16,8 @@ namespace {
 
 using namespace device::amd;
 
-constexpr int kThreads = 256;
-constexpr int kPerLane = 8; // elements
-
-struct Side { // keys or values
-    const uint8_t *codes, *scales;
-    void *to;
-    int64_t code_block, code_head, code_row;    // bytes
-    int64_t scale_block, scale_head, scale_row; // bytes
-    int64_t token_stride, head_stride;          // elements
-    uint32_t lanes_per_row;                     // size / 8
-};
-
-struct ReadArgs {
-    Side k, v;
-    const int64_t *slot_mapping;
-    int64_t num_slots;
-    uint32_t num_tokens;
-    uint32_t k_lanes;     // of a token: heads x k.lanes_per_row
-    uint32_t token_lanes; // of its keys and values
-    uint32_t block_tokens; // tokens of a workgroup
-    uint32_t block_size;
-    int32_t block_shift;  // log2(block_size) when it is a power of two, else -1
-};
+using Lane = fp4::RowLane<const uint8_t, void>;
+using Args = fp4::RowArgs<const uint8_t, void>;
 
 // Eight values as they are stored.
 struct EightBF16 {
@@ -77,47 +58,47 @@ struct EightF32 {
 };
 
 // ALIGNED: outputs at multiples of 16 bytes, rows of codes at multiples of 4; otherwise element by element, byte by byte.
-template <typename Eight, bool ALIGNED>
-__global__ void __launch_bounds__(kThreads) pagedReadingFp4Kernel(ReadArgs a) {
-    const uint32_t first = blockIdx.x * a.block_tokens;
-    const uint32_t lanes = min(a.block_tokens, a.num_tokens - first) * a.token_lanes;
-    for (uint32_t at = threadIdx.x; at < lanes; at += kThreads) {
-        const uint32_t t = at / a.token_lanes;
-        uint32_t u = at - t * a.token_lanes;
-        const bool value = u >= a.k_lanes;
-        u -= value ? a.k_lanes : 0;
-        const Side &side = value ? a.v : a.k;
-        const uint32_t head = u / side.lanes_per_row, chunk = u - head * side.lanes_per_row;
-        const uint32_t token = first + t;
-        const int64_t slot = a.slot_mapping[token];
-        uint32_t codes = 0, scale = 0;
-        if (slot >= 0 && slot < a.num_slots) {
-            const int64_t page = a.block_shift >= 0 ? slot >> a.block_shift : slot / a.block_size;
-            const int64_t row = slot - page * a.block_size;
-            const uint8_t *from = side.codes + page * side.code_block + head * side.code_head + row * side.code_row + chunk * 4;
+template <typename Eight, bool ALIGNED, int ROUNDS>
+__global__ void __launch_bounds__(fp4::kRowThreads) pagedReadingFp4Kernel(Args a) {
+    const Lane lane(a, ROUNDS);
+    if (!lane.exists || lane.token >= a.num_tokens) {
+        return;
+    }
+    int64_t slot[ROUNDS];
+    uint32_t codes[ROUNDS], scale[ROUNDS];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        slot[i] = a.slot_mapping[min(lane.token + i * a.token_groups, a.num_tokens - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        codes[i] = scale[i] = 0;
+        if (slot[i] >= 0 && slot[i] < a.num_slots) {
+            int64_t page, row;
+            Lane::place(a, slot[i], page, row);
+            const uint8_t *from = lane.codes + page * lane.code_block + row * lane.code_row;
             if constexpr (ALIGNED) {
-                codes = loadStreamed<uint32_t>(from);
+                codes[i] = loadStreamed<uint32_t>(from);
             } else {
-                codes = from[0] | from[1] << 8 | from[2] << 16 | static_cast<uint32_t>(from[3]) << 24;
+                codes[i] = from[0] | from[1] << 8 | from[2] << 16 | static_cast<uint32_t>(from[3]) << 24;
             }
-            scale = side.scales[page * side.scale_block + head * side.scale_head + row * side.scale_row + (chunk >> 2)];
-        }
-        Eight eight;
-        eight.of(codes, mx::scaleOf(scale));
-        auto *to = static_cast<typename Eight::Element *>(side.to) + token * side.token_stride + head * side.head_stride
-                 + chunk * kPerLane;
-        if constexpr (ALIGNED) {
-            eight.store(to);
-        } else {
-            eight.storeEach(to);
+            scale[i] = lane.scales[page * lane.scale_block + row * lane.scale_row];
         }
     }
-}
-
-Side sideOf(const void *codes, const void *scales, void *to, const fp4::PoolStrides &c, const fp4::PoolStrides &s,
-            ptrdiff_t token_stride, ptrdiff_t head_stride, size_t size) {
-    return Side{static_cast<const uint8_t *>(codes), static_cast<const uint8_t *>(scales), to, c.block, c.head, c.row,
-                s.block, s.head, s.row, token_stride, head_stride, static_cast<uint32_t>(size / kPerLane)};
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        const uint32_t token = lane.token + i * a.token_groups;
+        if (token < a.num_tokens) {
+            Eight eight;
+            eight.of(codes[i], mx::scaleOf(scale[i]));
+            auto *to = static_cast<typename Eight::Element *>(lane.wide) + token * lane.token_stride + lane.in_token;
+            if constexpr (ALIGNED) {
+                eight.store(to);
+            } else {
+                eight.storeEach(to);
+            }
+        }
+    }
 }
 
 } // namespace
@@ -170,29 +151,20 @@ infiniStatus_t Descriptor::calculate(void *workspace, size_t workspace_size, voi
         return INFINI_STATUS_BAD_PARAM; // a base address that is not aligned to the element size
     }
 
-    ReadArgs a{};
-    a.k = sideOf(k_codes, k_scales, k, pool.k_codes, pool.k_scales, in.k_token_stride, in.k_head_stride, pool.k_size);
-    a.v = sideOf(v_codes, v_scales, v, pool.v_codes, pool.v_scales, in.v_token_stride, in.v_head_stride, pool.v_size);
-    a.slot_mapping = static_cast<const int64_t *>(slot_mapping);
-    a.num_slots = static_cast<int64_t>(pool.num_blocks) * static_cast<int64_t>(pool.block_size);
-    a.num_tokens = static_cast<uint32_t>(in.num_tokens);
-    a.k_lanes = static_cast<uint32_t>(pool.num_kv_heads) * a.k.lanes_per_row;
-    a.token_lanes = a.k_lanes + static_cast<uint32_t>(pool.num_kv_heads) * a.v.lanes_per_row;
-    a.block_tokens = a.token_lanes >= kThreads ? 1 : kThreads / a.token_lanes;
-    a.block_size = static_cast<uint32_t>(pool.block_size);
-    a.block_shift = a.block_size > 0 && (a.block_size & (a.block_size - 1)) == 0 ? __builtin_ctz(a.block_size) : -1;
-
-    const uint64_t targets = address(k) | address(v)
-                           | (static_cast<uint64_t>(in.k_token_stride | in.k_head_stride | in.v_token_stride | in.v_head_stride) * es);
-    const bool aligned = targets % 16 == 0 && (address(k_codes) | address(v_codes)) % 4 == 0 && pool.codeRowsAligned(4);
-    const uint32_t grid = (a.num_tokens + a.block_tokens - 1) / a.block_tokens;
+    auto bytes = [](const void *p) { return static_cast<const uint8_t *>(p); };
+    const auto l = fp4::rowLaunch(in, bytes(k_codes), bytes(v_codes), bytes(k_scales), bytes(v_scales), k, v, slot_mapping, es,
+                                  device::amd::deviceInfo(device_id).compute_units);
     auto stream = static_cast<hipStream_t>(stream_);
     auto launch = [&](auto eight) {
         using Eight = decltype(eight);
-        if (aligned) {
-            pagedReadingFp4Kernel<Eight, true><<<grid, kThreads, 0, stream>>>(a);
+        if (!l.aligned) {
+            pagedReadingFp4Kernel<Eight, false, 1><<<l.grid, fp4::kRowThreads, 0, stream>>>(l.args);
+        } else if (l.rounds == 4) {
+            pagedReadingFp4Kernel<Eight, true, 4><<<l.grid, fp4::kRowThreads, 0, stream>>>(l.args);
+        } else if (l.rounds == 2) {
+            pagedReadingFp4Kernel<Eight, true, 2><<<l.grid, fp4::kRowThreads, 0, stream>>>(l.args);
         } else {
-            pagedReadingFp4Kernel<Eight, false><<<grid, kThreads, 0, stream>>>(a);
+            pagedReadingFp4Kernel<Eight, true, 1><<<l.grid, fp4::kRowThreads, 0, stream>>>(l.args);
         }
     };
     switch (in.dtype) {
