@@ -2,16 +2,20 @@
 // 256.
 //
 // A wavefront takes the up to 16 query heads of one KV head together and walks a run of tokens in steps of 32 (two tiles of
-// 16), so that every byte of the pool is read once. lane = 16 g + c (g = 0..3, c = 0..15). Per tile:
-//   S[token][head] = K . Q^T   v_mfma_f32_16x16x32, A = K: lane c holds HEAD / 4 neighbouring elements of one token, straight
-//                              from the load. The matrix instruction sums over the elements whatever their order, as long as
-//                              the query has the same, so a lane's elements need not be spread over the four groups g, and
-//                              each lane's codes lie under one scale (two above head 128).
-//   O[head][dim] += P . V      v_mfma_f32_16x16x32 over both tiles of a step, A = P as S came out, B = V: the lane that loads
-//                              a strip of columns of tokens 4 i + g (i = 0..3) is the lane that feeds those to the matrix
-//                              unit; pairs of tokens are interleaved with byte permutes.
-// So nothing passes through LDS. Row m of a tile is token 4 (m % 4) + m / 4: the accumulator rows of group g are then tokens
-// g, 4 + g, 8 + g, 12 + g, and each V load instruction covers four neighbouring rows.
+// 16), so that every byte of the pool is read once. Codes and scales go from global memory straight into the wavefront's own
+// piece of LDS (global_load_lds, no register in between), several steps ahead: a step is 4.4 KB at head 128, and at the rate
+// of the memory some 25 KB per compute unit have to be in flight for every microsecond that a load takes. (Held in registers
+// instead, 26 of them a step, one step ahead was all there was room for: 128 sequences of 1 024 - 8 192, 64 / 8 heads of 128,
+// 151 us, 4.3 TB/s.) lane = 16 g + c (g = 0..3, c = 0..15). Per tile:
+//   S[token][head] = K . Q^T   v_mfma_f32_16x16x32, A = K: lane c holds HEAD / 4 neighbouring elements of one token. The
+//                              matrix instruction sums over the elements whatever their order, as long as the query has the
+//                              same, so a lane's elements need not be spread over the four groups g, and each lane's codes
+//                              lie under one scale (two above head 128).
+//   O[head][dim] += P . V      v_mfma_f32_16x16x32 over both tiles of a step, A = P as S came out, B = V: a lane reads a
+//                              strip of columns of tokens 4 i + g (i = 0..3) of either tile; pairs of tokens are interleaved
+//                              with byte permutes.
+// Row m of a tile is token 4 (m % 4) + m / 4: the accumulator rows of group g are then tokens g, 4 + g, 8 + g, 12 + g, and
+// the four groups read four neighbouring rows of V.
 //
 // Codes become bf16 or fp16 under their scale by v_cvt_scalef32_pk_*, two elements per instruction: K in the query's type, V
 // in fp16, where every written value is exact and the probabilities keep eleven bits (as bf16 they would add an error as large
@@ -36,17 +40,18 @@ using op::paged_attention::amd::fastExp2;
 using op::paged_attention::amd::Half;
 using op::paged_attention::amd::kHeadsPerWave;
 using op::paged_attention::amd::kLog2e;
+using op::paged_attention::amd::loadLane16ToLds;
 using op::paged_attention::amd::maxAcrossTokenGroups;
 using op::paged_attention::amd::maxOf;
-using op::paged_attention::amd::sumAcrossTokenGroups;
 using op::paged_attention::amd::TileBF16;
 using op::paged_attention::amd::TileF16;
 using op::paged_attention::amd::waveInclusiveSum;
+using op::paged_attention::amd::waveMaxInt;
 namespace mx = device::amd::mx;
 
 constexpr int kStepTokens = 32;
 constexpr int kDecodeThreads = 256;  // four wavefronts that share nothing but the launch
-constexpr int kLeastSteps = 4;       // of a run: below that the merge costs more than it saves
+constexpr int kLeastSteps = 1;       // of a run
 constexpr float kLazyLog2 = 8.0f;    // how far (in powers of two) a maximum may outgrow its reference point
 
 enum class IndexType : int32_t { i64, i32, u32 };
@@ -72,18 +77,22 @@ struct DecodeFp4Args {
     PoolSide k_codes, k_scales, v_codes, v_scales;
     const void *block_tables;
     const void *seq_lens;
+    const void *cu_seqlens_q;  // RUNS: [num_seqs + 1] prefix sums of the query tokens; otherwise one each
     const float *alibi_slopes; // nullptr = no ALiBi
     IndexType index_type;
 
-    // partial results, two places per run: [stream][run][0 = of a sequence that began before it, 1 = of one that ends behind it]
-    float *part_acc;  // [..][part_rows][HEAD]
-    float2 *part_ml;  // [..][part_rows] reference point (log2), denominator
-    int32_t part_rows; // heads of a chunk: min(group, 16)
+    // partial results, two places per run: [stream][run][0 = of a segment that began before it, 1 = of one that ends behind it]
+    float *part_acc;   // [..][part_rows][HEAD]
+    float2 *part_ml;   // [..][part_rows] reference point (log2), denominator
+    int4 *segments;    // first run, last run, sequence, chunk; written where a segment begins
+    int32_t *num_segments; // RUNS
+    int32_t part_rows; // of a segment: min(group, 16); RUNS: 16
 
     float scale_log2; // scale * log2(e)
     int32_t num_seqs, num_heads, num_kv_heads;
+    int32_t total_q_tokens;
     int32_t group;       // query heads per KV head
-    int32_t head_chunks; // of up to 16 query heads
+    int32_t head_chunks; // of up to 16 query heads; RUNS: 1
     int32_t runs;        // per stream (KV head and chunk), at most
     int32_t block_size;
     int32_t num_blocks;  // pool size; table entries are clamped into [0, num_blocks)
@@ -95,30 +104,69 @@ struct DecodeFp4Args {
     int64_t block_table_stride;
 };
 
-// Tokens of sequence `seq`, forced into what its table can hold.
-__device__ __forceinline__ int sequenceTokens(const DecodeFp4Args &a, int seq) {
-    const int64_t n = loadIndexOf(a.index_type, a.seq_lens, seq);
-    return static_cast<int>(n < 0 ? 0 : (n > a.capacity ? a.capacity : n));
+// What a wavefront needs before its first memory request can go out. It stands in front of the kernel's arguments: the file is
+// compiled with -amdgpu-kernarg-preload-count=8, which has the dispatcher put these eight words into scalar registers.
+struct DecodeFp4Kernarg {
+    const void *seq_lens;
+    const void *cu_seqlens_q;
+    int32_t index_type, num_seqs, capacity, runs;
+    DecodeFp4Args a;
+};
+// The same arguments, read again: what a call needs once in a thousand tokens does not live in scalar registers in between
+// (there are not enough: kept, they were spilled into vector registers and read back from there).
+typedef const __attribute__((address_space(4))) DecodeFp4Args *ArgsAgain;
+__device__ __forceinline__ ArgsAgain argsAgain() {
+    auto p = (const __attribute__((address_space(4))) DecodeFp4Kernarg *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return &p->a;
 }
+
 __device__ __forceinline__ int stepsOf(int tokens) { return (tokens + kStepTokens - 1) / kStepTokens; }
 
-// The runs that `steps` steps are cut into: run i has steps [i steps / runs, (i + 1) steps / runs).
-__device__ __forceinline__ int runsFor(const DecodeFp4Args &a, int64_t steps) {
-    const int64_t most = (steps + kLeastSteps - 1) / kLeastSteps;
-    return static_cast<int>(most < a.runs ? most : a.runs);
-}
-__device__ __forceinline__ int64_t runStart(int64_t steps, int runs, int run) { return steps * run / runs; }
-__device__ __forceinline__ int runOf(int64_t steps, int runs, int64_t step) { return static_cast<int>(((step + 1) * runs - 1) / steps); }
-
-// Steps of all sequences.
-__device__ __forceinline__ int64_t totalSteps(const DecodeFp4Args &a, int lane) {
-    int64_t total = 0;
-    for (int base = 0; base < a.num_seqs; base += 64) {
-        const int n = base + lane < a.num_seqs ? stepsOf(sequenceTokens(a, base + lane)) : 0;
-        total += __builtin_amdgcn_readlane(waveInclusiveSum(n), 63);
+// The work of one sequence: `segments` times `steps` steps. RUNS: a segment is 16 rows, a row a (query token, head of the group)
+// pair, token-major; query token j is row q_start + j of q and sees history + j + 1 tokens. Otherwise one segment, the heads.
+struct Work {
+    int tokens; // forced into what the table can hold
+    int segments, steps;
+    int q_start, q_len, history; // RUNS
+    __device__ __forceinline__ int all() const { return segments * steps; }
+};
+template <bool RUNS>
+__device__ __forceinline__ Work workOf(IndexType type, const void *seq_lens, const void *cu, int capacity, int total_q, int group, int seq) {
+    const int64_t kv = loadIndexOf(type, seq_lens, seq);
+    Work w{};
+    w.tokens = static_cast<int>(kv < 0 ? 0 : (kv > capacity ? capacity : kv));
+    w.steps = stepsOf(w.tokens);
+    w.segments = 1;
+    if constexpr (RUNS) { // clipped to the query and the table, so that inconsistent lengths cannot reach outside the operands
+        int64_t q0 = loadIndexOf(type, cu, seq), q1 = loadIndexOf(type, cu, seq + 1);
+        const int64_t lim = int64_t(1) << 30;
+        int64_t history = kv - (q1 - q0);
+        history = history < -lim ? -lim : (history > lim ? lim : history);
+        q0 = q0 < 0 ? 0 : (q0 > total_q ? total_q : q0);
+        q1 = q1 < q0 ? q0 : (q1 > total_q ? total_q : q1);
+        w.q_start = static_cast<int>(q0);
+        w.q_len = static_cast<int>(q1 - q0);
+        w.history = static_cast<int>(history);
+        w.segments = (w.q_len * group + kHeadsPerWave - 1) / kHeadsPerWave;
     }
-    return total;
+    return w;
 }
+
+// The runs that `steps` steps (fewer than 2^31) are cut into: the first steps % runs have one more than the others.
+__device__ __forceinline__ uint32_t runsFor(uint32_t most, uint32_t steps) {
+    const uint32_t runs = (steps + kLeastSteps - 1) / kLeastSteps;
+    return runs < most ? runs : most;
+}
+struct Cut {
+    uint32_t least, more; // steps of a run; how many have one more
+    __device__ __forceinline__ Cut(uint32_t steps, uint32_t runs) : least(steps / runs), more(steps - least * runs) {}
+    __device__ __forceinline__ uint32_t start(uint32_t run) const { return run * least + (run < more ? run : more); }
+    __device__ __forceinline__ uint32_t runOf(uint32_t step) const { // that has step `step`
+        const uint32_t border = more * (least + 1);
+        return step < border ? step / (least + 1) : more + (step - border) / least;
+    }
+};
 
 template <int BYTES> struct Bits;
 template <> struct Bits<2> { using type = uint16_t; };
@@ -140,9 +188,9 @@ __device__ __forceinline__ void loadWords(const char *p, uint32_t *to) {
     }
 }
 
-// How a head's elements and columns lie in the lanes. K: pieces of 128 (32 elements a lane, one 16-byte load) and, at 64
-// and 192, one of 64 (16 elements, 8 bytes). V: one strip of HEAD / 16 neighbouring columns a lane, at head 192 a strip of
-// 8 columns out of the first 128 and one of 4 out of the rest, so that no lane reads three bytes of two words.
+// How a head's elements and columns lie in the lanes. K: pieces of 128 (32 elements a lane) and, at 64 and 192, one of 64 (16
+// elements). V: one strip of HEAD / 16 neighbouring columns a lane, at head 192 a strip of 8 columns out of the first 128 and
+// one of 4 out of the rest, so that no lane reads three bytes of two words.
 template <int HEAD>
 struct Layout {
     static constexpr int kWords = HEAD / 32;                   // dwords of K codes a lane and token
@@ -152,151 +200,210 @@ struct Layout {
     static constexpr int kCols = HEAD / 16;
     static constexpr int kVWords = HEAD == 64 || HEAD == 128 ? 1 : 2;
     static constexpr bool pieceWhole(int p) { return 128 * p + 128 <= HEAD; }
-    // first element and scale of lane group g in piece p
+    // first element of lane group g in piece p
     static __device__ __forceinline__ int element(int p, int g) { return 128 * p + (pieceWhole(p) ? 32 : 16) * g; }
     // first column of lane c in strip s
     static __device__ __forceinline__ int column(int s, int c) { return s == 0 ? kStripCols * c : 128 + 4 * c; }
+
+    // In LDS: rows of 16-byte chunks of codes; those of K are exchanged by the row, so that reads of one chunk of 16 rows meet
+    // in no bank.
+    static constexpr int kChunks = HEAD / 32;
+    static __device__ __forceinline__ int kSlot(int row, int chunk) {
+        return row * kChunks + (chunk ^ (((row & 15) * kChunks / 16) & (HEAD == 192 ? 1 : kChunks - 1)));
+    }
+    // Load instructions of a step: codes (of K, of V), scales of K, of V.
+    static constexpr int kCodeLoads = HEAD / 64, kKScaleLoads = 2 * kPieces, kVScaleLoads = HEAD / 64;
+    static constexpr int kLoads = 2 * kCodeLoads + kKScaleLoads + kVScaleLoads;
+    // Workgroups (of four wavefronts) that share a compute unit, and the steps in flight or at hand that its 160 KiB of LDS
+    // then hold for each wavefront.
+    static constexpr int kPerUnit = HEAD == 64 ? 3 : (HEAD == 128 ? 3 : 2);
+    static constexpr int kStages = HEAD == 64 ? 4 : 2;
 };
 
-// What a lane loads of one step.
+// One step in LDS. A scale has a dword of its own: K [tile][piece][lane], V [tile][group g][scale of the row][i].
 template <int HEAD>
 struct Step {
     using L = Layout<HEAD>;
-    uint32_t k[2][L::kWords];
-    uint8_t ks[2][L::kPieces];
-    uint32_t v[8][L::kVWords]; // [tile][i]: token 4 i + g
-    uint8_t vs[8][L::kStrips];
+    uint4 k[64 * L::kCodeLoads], v[64 * L::kCodeLoads];
+    uint32_t ks[64 * L::kKScaleLoads], vs[64 * L::kVScaleLoads];
 };
 
-// Where the rows of a sequence lie. GRAIN: the page size is a multiple of this many tokens; 16 = a tile lies in one page, 8 =
-// each half of it does, 1 = every lane looks its rows up for itself.
+// From global memory straight into LDS, as loadLane16ToLds does for 16 bytes: a byte of each lane, widened to a dword. Lane i
+// writes lds_base + 4 i.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ uint32_t ldsAddress(const void *p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)p));
+}
+__device__ __forceinline__ void loadByteToLds(const char *uniform_base, uint32_t lane_offset, uint32_t *lds_base) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, %1 nt"
+                 :: "v"(lane_offset), "s"(uniform_base), "s"(ldsAddress(lds_base)) : "memory", "m0");
+}
+__device__ __forceinline__ void loadByteToLds(const char *lane_pointer, uint32_t *lds_base) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off nt"
+                 :: "v"(lane_pointer), "s"(ldsAddress(lds_base)) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// All but the last LEFT of this wavefront's vector memory operations are done.
+template <int LEFT>
+__device__ __forceinline__ void waitLoads() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(LEFT) : "memory"); }
+// Its reads out of LDS have delivered: what they read may be overwritten.
+__device__ __forceinline__ void waitLdsReads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// Where the rows of a sequence lie, and their loads. GRAIN: the page size is a multiple of this many tokens; 16 = a tile lies in
+// one page, 8 = each half of it does, 1 = rows are looked up one by one.
 template <int HEAD, int GRAIN>
 struct Pages {
     using L = Layout<HEAD>;
-    const DecodeFp4Args &a;
-    int lane, g, c, kv_head;
+    static constexpr int kUnits = GRAIN > 1 ? kStepTokens / GRAIN : 1; // of a step
+    int lane, kv_head, block_size;
+    int32_t k_code_row, k_scale_row, v_code_row, v_scale_row; // bytes
     int64_t table;  // index of the sequence's first table entry
     int tokens;     // of the sequence
-    // GRAIN > 1: the pages of 64 table entries, one a lane, and the unit (GRAIN tokens) that comes next
+    int token;      // that the next step begins with
+    // GRAIN > 1: where the pages of 64 table entries begin, one a lane; entry and row of the unit (GRAIN tokens) that comes next
+    uint64_t k_code_page, k_scale_page, v_code_page, v_scale_page;
+    int first_entry, entry;
+    // GRAIN = 1: page and row of token `token + lane % 32`
     int32_t ids;
-    int first_entry, entry, row, token;
+    int row;
 
-    __device__ __forceinline__ int32_t page(int64_t at) const {
-        return clampPage(loadIndexOf(a.index_type, a.block_tables, table + at), a.num_blocks);
+    __device__ __forceinline__ Pages(const DecodeFp4Args &a, int lane_, int kv_head_)
+        : lane(lane_), kv_head(kv_head_), block_size(a.block_size), k_code_row(a.k_codes.row), k_scale_row(a.k_scales.row),
+          v_code_row(a.v_codes.row), v_scale_row(a.v_scales.row) {}
+
+    __device__ __forceinline__ int32_t page(ArgsAgain a, int64_t at) const {
+        return clampPage(loadIndexOf(a->index_type, a->block_tables, table + at), a->num_blocks);
+    }
+    template <typename Side> // PoolSide, in the arguments' address space
+    __device__ __forceinline__ const char *rowOf(const Side &s, int32_t id, int r) const {
+        return s.base + id * s.block + kv_head * s.head + static_cast<int64_t>(r) * s.row;
     }
     __device__ __forceinline__ void fetch(int from) {
+        const ArgsAgain a = argsAgain();
         first_entry = from;
-        const int last = (tokens - 1) / a.block_size;
-        ids = page(min(from + lane, last));
+        const int last = (tokens - 1) / block_size;
+        const int32_t id = page(a, min(from + lane, last));
+        k_code_page = reinterpret_cast<uint64_t>(rowOf(a->k_codes, id, 0));
+        k_scale_page = reinterpret_cast<uint64_t>(rowOf(a->k_scales, id, 0));
+        v_code_page = reinterpret_cast<uint64_t>(rowOf(a->v_codes, id, 0));
+        v_scale_page = reinterpret_cast<uint64_t>(rowOf(a->v_scales, id, 0));
     }
-    __device__ __forceinline__ void begin(int seq, int tokens_, int step) {
-        table = seq * a.block_table_stride;
+    static __device__ __forceinline__ const char *ofLane(uint64_t x, int lane, uint32_t offset) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(x), lane);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(x >> 32), lane);
+        return reinterpret_cast<const char *>((static_cast<uint64_t>(hi) << 32 | lo) + offset);
+    }
+    __device__ __forceinline__ void lookUp() {
+        const int t = min(token + (lane & 31), tokens - 1);
+        const int e = t / block_size;
+        row = t - e * block_size;
+        ids = page(argsAgain(), e);
+    }
+    __device__ __forceinline__ void begin(int64_t table_, int tokens_, int step) {
+        table = table_;
         tokens = tokens_;
         token = step * kStepTokens;
         if constexpr (GRAIN > 1) {
-            entry = token / a.block_size;
-            row = token - entry * a.block_size;
+            entry = token / block_size;
+            row = token - entry * block_size;
             fetch(entry);
+        } else {
+            lookUp();
         }
     }
-    static __device__ __forceinline__ const char *rowOf(const PoolSide &s, int32_t page, int kv_head, int row) {
-        return s.base + page * s.block + kv_head * s.head + static_cast<int64_t>(row) * s.row;
-    }
 
-    struct Unit {
-        const char *kc, *ks, *vc, *vs;
+    // One of the pool's tensors over the step at hand: the first row of each unit (the same in all lanes).
+    struct Units {
+        const char *base[kUnits];
     };
-    // The next GRAIN tokens; where the sequence has none left, the last ones again.
-    __device__ __forceinline__ Unit next() {
-        if (entry - first_entry >= 64) {
-            fetch(entry);
-        }
-        const int32_t id = __builtin_amdgcn_readlane(ids, entry - first_entry);
-        const Unit u{rowOf(a.k_codes, id, kv_head, row), rowOf(a.k_scales, id, kv_head, row), rowOf(a.v_codes, id, kv_head, row),
-                     rowOf(a.v_scales, id, kv_head, row)};
-        token += GRAIN;
-        if (token < tokens) {
-            row += GRAIN;
-            if (row >= a.block_size) {
-                row = 0;
-                ++entry;
-            }
-        }
-        return u;
-    }
-
-    __device__ __forceinline__ void loadK(Step<HEAD> &to, int tile, const char *codes, const char *scales) const {
+    // The lane's byte at `column` of row `token_in_step`, which lies in one of the units FIRST .. LAST.
+    template <int FIRST, int LAST>
+    __device__ __forceinline__ const char *pick(const Units &u, int unit) const {
+        const char *p = u.base[FIRST];
 #pragma unroll
-        for (int p = 0; p < L::kPieces; ++p) {
-            const int e = L::element(p, g);
-            if (L::pieceWhole(p)) {
-                loadWords<16>(codes + e / 2, &to.k[tile][4 * p]);
+        for (int i = FIRST + 1; i <= LAST; ++i) {
+            p = unit >= i ? u.base[i] : p;
+        }
+        return p;
+    }
+    // load16 / loadByte of every lane's (row of the step, byte of the row); rows lie between FIRST_ROW and LAST_ROW.
+    template <int FIRST_ROW, int LAST_ROW, typename Load>
+    __device__ __forceinline__ void each(const PoolSide DecodeFp4Args::*side, int32_t row_bytes, const Units &u, int row_of_step, int byte,
+                                         Load load) const {
+        if constexpr (GRAIN > 1) {
+            constexpr int first = FIRST_ROW / GRAIN, last = LAST_ROW / GRAIN;
+            const uint32_t offset = static_cast<uint32_t>((row_of_step % GRAIN) * row_bytes + byte);
+            if constexpr (first == last) {
+                load(u.base[first], offset);
             } else {
-                loadWords<8>(codes + e / 2, &to.k[tile][4 * p]);
-            }
-            to.ks[tile][p] = __builtin_nontemporal_load(reinterpret_cast<const uint8_t *>(scales + e / 32));
-        }
-    }
-    __device__ __forceinline__ void loadV(Step<HEAD> &to, int at, const char *codes, const char *scales) const {
-#pragma unroll
-        for (int s = 0; s < L::kStrips; ++s) {
-            const int d = L::column(s, c);
-            if (s == 0) {
-                loadWords<L::kStripCols / 2>(codes + d / 2, to.v[at]);
-            } else {
-                loadWords<2>(codes + d / 2, &to.v[at][1]);
-            }
-            to.vs[at][s] = __builtin_nontemporal_load(reinterpret_cast<const uint8_t *>(scales + d / 32));
-        }
-    }
-
-    // The 32 tokens that come next.
-    __device__ __forceinline__ void load(Step<HEAD> &to) {
-        const int m = 4 * (c & 3) + (c >> 2); // this lane's K row of a tile
-        if constexpr (GRAIN == 16) {
-#pragma unroll
-            for (int tile = 0; tile < 2; ++tile) {
-                const Unit u = next();
-                loadK(to, tile, u.kc + m * a.k_codes.row, u.ks + m * a.k_scales.row);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    loadV(to, 4 * tile + i, u.vc + 4 * i * a.v_codes.row + g * a.v_codes.row,
-                          u.vs + 4 * i * a.v_scales.row + g * a.v_scales.row);
-                }
-            }
-        } else if constexpr (GRAIN == 8) {
-#pragma unroll
-            for (int tile = 0; tile < 2; ++tile) {
-                const Unit u = next(), w = next();
-                const bool second = m >= 8;
-                loadK(to, tile, (second ? w.kc : u.kc) + (m & 7) * a.k_codes.row, (second ? w.ks : u.ks) + (m & 7) * a.k_scales.row);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const Unit &x = i < 2 ? u : w;
-                    const int r = 4 * (i & 1) + g;
-                    loadV(to, 4 * tile + i, x.vc + r * a.v_codes.row, x.vs + r * a.v_scales.row);
-                }
+                load(pick<first, last>(u, row_of_step / GRAIN) + offset);
             }
         } else {
+            load(rowOf(argsAgain()->*side, __shfl(ids, row_of_step, 64), __shfl(row, row_of_step, 64)) + byte);
+        }
+    }
+
+    // The 32 tokens that come next; where the sequence has fewer left, its last rows again (GRAIN > 1: its last unit).
+    __device__ __forceinline__ void load(Step<HEAD> &to) {
+        Units kc, ks, vc, vs;
+        if constexpr (GRAIN > 1) {
 #pragma unroll
-            for (int tile = 0; tile < 2; ++tile) {
-                auto place = [&](int t, int32_t &id, int &r) {
-                    t = min(t, tokens - 1);
-                    const int e = t / a.block_size;
-                    r = t - e * a.block_size;
-                    id = page(e);
-                };
-                int32_t id;
-                int r;
-                place(token + 16 * tile + m, id, r);
-                loadK(to, tile, rowOf(a.k_codes, id, kv_head, r), rowOf(a.k_scales, id, kv_head, r));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    place(token + 16 * tile + 4 * i + g, id, r);
-                    loadV(to, 4 * tile + i, rowOf(a.v_codes, id, kv_head, r), rowOf(a.v_scales, id, kv_head, r));
+            for (int u = 0; u < kUnits; ++u) {
+                if (entry - first_entry >= 64) {
+                    fetch(entry);
+                }
+                const int in = entry - first_entry;
+                kc.base[u] = ofLane(k_code_page, in, static_cast<uint32_t>(row * k_code_row));
+                ks.base[u] = ofLane(k_scale_page, in, static_cast<uint32_t>(row * k_scale_row));
+                vc.base[u] = ofLane(v_code_page, in, static_cast<uint32_t>(row * v_code_row));
+                vs.base[u] = ofLane(v_scale_page, in, static_cast<uint32_t>(row * v_scale_row));
+                if (token + (u + 1) * GRAIN < tokens) {
+                    row += GRAIN;
+                    if (row >= block_size) {
+                        row = 0;
+                        ++entry;
+                    }
                 }
             }
-            token += kStepTokens;
+        }
+        struct Chunk {
+            uint4 *to;
+            __device__ __forceinline__ void operator()(const char *base, uint32_t offset) const { loadLane16ToLds<true>(base, offset, to); }
+            __device__ __forceinline__ void operator()(const char *p) const { loadLane16ToLds<true>(p, to); }
+        };
+        struct Byte {
+            uint32_t *to;
+            __device__ __forceinline__ void operator()(const char *base, uint32_t offset) const { loadByteToLds(base, offset, to); }
+            __device__ __forceinline__ void operator()(const char *p) const { loadByteToLds(p, to); }
+        };
+        constexpr int C = L::kChunks, kScales = HEAD / 32;
+        const int g = lane >> 4, c = lane & 15;
+        waitLdsReads();
+        auto codes = [&](auto j) {
+            constexpr int J = decltype(j)::value;
+            constexpr int first = 64 * J / C, last = (64 * J + 63) / C;
+            const int r = (64 * J + lane) / C, at = (64 * J + lane) % C;
+            each<first, last>(&DecodeFp4Args::k_codes, k_code_row, kc, r, 16 * (L::kSlot(r, at) - r * C), Chunk{to.k + 64 * J}); // (exchanged twice is back)
+            each<first, last>(&DecodeFp4Args::v_codes, v_code_row, vc, r, 16 * at, Chunk{to.v + 64 * J});
+            // V scales: 4 kScales entries for each of the eight (tile, group) pairs
+            const int e = 64 * J + lane, pair = e / (4 * kScales), scale = e % (4 * kScales) / 4, i = e & 3;
+            constexpr int first_tile = 64 * J / (16 * kScales), last_tile = (64 * J + 63) / (16 * kScales);
+            each<16 * first_tile, 16 * last_tile + 15>(&DecodeFp4Args::v_scales, v_scale_row, vs, 16 * (pair >> 2) + 4 * i + (pair & 3), scale, Byte{to.vs + 64 * J});
+        };
+        codes(std::integral_constant<int, 0>{});
+        if constexpr (L::kCodeLoads > 1) { codes(std::integral_constant<int, 1>{}); }
+        if constexpr (L::kCodeLoads > 2) { codes(std::integral_constant<int, 2>{}); }
+        if constexpr (L::kCodeLoads > 3) { codes(std::integral_constant<int, 3>{}); }
+        const int m = 4 * (c & 3) + (c >> 2);
+#pragma unroll
+        for (int p = 0; p < L::kPieces; ++p) {
+            each<0, 15>(&DecodeFp4Args::k_scales, k_scale_row, ks, m, L::element(p, g) / 32, Byte{to.ks + 64 * p});
+            each<16, 31>(&DecodeFp4Args::k_scales, k_scale_row, ks, 16 + m, L::element(p, g) / 32, Byte{to.ks + 64 * (L::kPieces + p)});
+        }
+        token += kStepTokens;
+        if constexpr (GRAIN == 1) {
+            lookUp();
         }
     }
 };
@@ -305,7 +412,9 @@ template <typename T, int HEAD>
 struct DecodeState {
     uint4 q[HEAD / 32];
     f32x4 o[HEAD / 16];
-    float m, l; // of head c: reference point of the exponentials (log2), this lane's part of the denominator
+    f32x4 l;         // denominators of rows 4 g .. 4 g + 3
+    float m, shift;  // of row c: reference point of the exponentials, in units of the raw product (PLAIN) or of log2; -m in log2
+                     // units, 0 while m = -inf (products that overflowed, all of them so far, have no weight, and are no NaN)
 };
 
 template <typename T>
@@ -315,13 +424,13 @@ __device__ __forceinline__ uint4 toQueryType<TileBF16>(uint32_t codes, float sca
 template <>
 __device__ __forceinline__ uint4 toQueryType<TileF16>(uint32_t codes, float scale) { return mx::toF16x8(codes, scale); }
 
-// Columns 2 B and 2 B + 1 of a strip: the operands of eight tokens each.
-template <int B, int HEAD>
-__device__ __forceinline__ void columnPair(const Step<HEAD> &s, const float (&scale)[8], int word, uint4 &even, uint4 &odd) {
+// Columns 2 B and 2 B + 1 of the eight in `codes`: the operands of eight tokens each.
+template <int B>
+__device__ __forceinline__ void columnPair(const uint32_t (&codes)[8], const float (&scale)[8], uint4 &even, uint4 &odd) {
     uint32_t w[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        w[j] = mx::toF16<B>(s.v[j][word], scale[j]);
+        w[j] = mx::toF16<B>(codes[j], scale[j]);
     }
     auto low = [](uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x05040100u); };
     auto high = [](uint32_t x, uint32_t y) { return __builtin_amdgcn_perm(y, x, 0x07060302u); };
@@ -329,45 +438,74 @@ __device__ __forceinline__ void columnPair(const Step<HEAD> &s, const float (&sc
     odd = make_uint4(high(w[0], w[1]), high(w[2], w[3]), high(w[4], w[5]), high(w[6], w[7]));
 }
 
-// One step. Tokens from `left` on are behind the sequence; what their rows hold has no part in anything.
-template <typename T, int HEAD>
-__device__ __forceinline__ void computeStep(const DecodeFp4Args &a, const Step<HEAD> &s, DecodeState<T, HEAD> &st, int g, int left,
-                                            float slope_log2, float away) {
+// What is the same for every step of a segment.
+struct Rows {
+    float scale_log2, slope_log2; // slope: of row c
+    float unit, lazy;             // log2 units in one of the maxima; kLazyLog2 in units of the maxima
+    bool plain;                   // no ALiBi and a positive scale: maxima are kept in units of the raw product
+    int visible;                  // tokens that row c sees
+    int least;                    // and the row of the segment that sees the fewest
+};
+
+// One step, from token t0 on. Tokens that a row does not see, and those behind the sequence, have no part in it, whatever their
+// rows of the pool hold.
+template <typename T, int HEAD, bool RUNS>
+__device__ __forceinline__ void computeStep(const Step<HEAD> &s, DecodeState<T, HEAD> &st, const Rows &rows, int lane, int t0, int tokens) {
     using L = Layout<HEAD>;
     constexpr bool kSplit = T::kSplitProbabilities == false; // fp16 outputs: two terms (see the top)
+    const int g = lane >> 4, c = lane & 15, k_row = 4 * (c & 3) + (c >> 2);
     f32x4 score[2];
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile) {
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < L::kWords; ++w) {
-            x = T::mfmaK32(toQueryType<T>(s.k[tile][w], mx::scaleOf(s.ks[tile][w / 4])), st.q[w], x);
+        for (int p = 0; p < L::kPieces; ++p) {
+            const float scale = mx::scaleOf(s.ks[64 * (L::kPieces * tile + p) + lane]);
+            const uint4 *row = s.k + 16 * tile * L::kChunks;
+            {
+                if (L::pieceWhole(p)) {
+                    const uint4 w = row[L::kSlot(k_row, 4 * p + g)];
+                    x = T::mfmaK32(toQueryType<T>(w.x, scale), st.q[4 * p], x);
+                    x = T::mfmaK32(toQueryType<T>(w.y, scale), st.q[4 * p + 1], x);
+                    x = T::mfmaK32(toQueryType<T>(w.z, scale), st.q[4 * p + (L::kWords > 2 ? 2 : 0)], x);
+                    x = T::mfmaK32(toQueryType<T>(w.w, scale), st.q[4 * p + (L::kWords > 2 ? 3 : 0)], x);
+                } else {
+                    const uint2 w = reinterpret_cast<const uint2 *>(row + L::kSlot(k_row, 4 * p + (g >> 1)))[g & 1];
+                    x = T::mfmaK32(toQueryType<T>(w.x, scale), st.q[4 * p], x);
+                    x = T::mfmaK32(toQueryType<T>(w.y, scale), st.q[4 * p + 1], x);
+                }
+            }
         }
-        score[tile] = x * a.scale_log2;
+        score[tile] = x;
     }
-    if (a.alibi_slopes != nullptr) {
+    auto tokenOf = [&](int j) { return 16 * (j / 4) + 4 * (j & 3) + g; }; // of the step
+    const bool masked = t0 + kStepTokens > (RUNS ? rows.least : tokens);
+    const int left = (RUNS ? rows.visible : tokens) - t0; // RUNS: of row c
+    if (!rows.plain) {
+        const float away = static_cast<float>(1 - left);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            score[j / 4][j & 3] += slope_log2 * (away + static_cast<float>(16 * (j / 4) + 4 * (j & 3) + g));
+            score[j / 4][j & 3] = score[j / 4][j & 3] * rows.scale_log2 + rows.slope_log2 * (away + static_cast<float>(tokenOf(j)));
         }
     }
-    if (left < kStepTokens) {
+    if (masked) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            score[j / 4][j & 3] = 16 * (j / 4) + 4 * (j & 3) + g < left ? score[j / 4][j & 3] : -INFINITY;
+            score[j / 4][j & 3] = tokenOf(j) < left ? score[j / 4][j & 3] : -INFINITY;
         }
     }
-    const float top = maxOf(maxOf(maxOf(score[0][0], score[0][1]), maxOf(score[0][2], score[0][3])),
-                            maxOf(maxOf(score[1][0], score[1][1]), maxOf(score[1][2], score[1][3])));
+    const float top = maxOf(maxOf(maxOf(maxOf(score[0][0], score[0][1]), score[0][2]), maxOf(score[0][3], score[1][0])),
+                            maxOf(maxOf(score[1][1], score[1][2]), score[1][3]));
     // (a NaN compares as not greater; it reaches the outputs by its own probability)
-    if (__builtin_amdgcn_ballot_w64(top > st.m + kLazyLog2) != 0) {
+    if (__builtin_amdgcn_ballot_w64(top > st.m + rows.lazy) != 0) {
         const float m = maxOf(st.m, maxAcrossTokenGroups(top));
-        const float alpha = st.m == m ? 1.0f : fastExp2(st.m - m);
-        st.l *= alpha;
+        const float alpha = m > st.m ? fastExp2((st.m - m) * rows.unit) : 1.0f;
         st.m = m;
+        st.shift = m == -INFINITY ? 0.0f : -m * rows.unit;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float f = __shfl(alpha, 4 * g + i, 64);
+            st.l[i] *= f;
 #pragma unroll
             for (int e = 0; e < L::kCols; ++e) {
                 st.o[e][i] *= f;
@@ -375,12 +513,10 @@ __device__ __forceinline__ void computeStep(const DecodeFp4Args &a, const Step<H
         }
     }
     float p[8];
-    const float from = st.m == -INFINITY ? 0.0f : st.m; // products that overflowed, all of them so far: no weight, not a NaN
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        p[j] = fastExp2(score[j / 4][j & 3] - from);
+        p[j] = fastExp2(__builtin_fmaf(score[j / 4][j & 3], rows.unit, st.shift));
     }
-    st.l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
     const uint4 hi = make_uint4(TileF16::pack2(p[0], p[1]), TileF16::pack2(p[2], p[3]), TileF16::pack2(p[4], p[5]),
                                 TileF16::pack2(p[6], p[7]));
     uint4 lo = make_uint4(0, 0, 0, 0);
@@ -388,71 +524,144 @@ __device__ __forceinline__ void computeStep(const DecodeFp4Args &a, const Step<H
         auto rest = [](float x, float y, uint32_t w) { return TileF16::pack2(x - TileF16::unpackLo(w), y - TileF16::unpackHi(w)); };
         lo = make_uint4(rest(p[0], p[1], hi.x), rest(p[2], p[3], hi.y), rest(p[4], p[5], hi.z), rest(p[6], p[7], hi.w));
     }
+    const uint4 ones = make_uint4(0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u); // fp16
+    st.l = TileF16::mfmaK32(hi, ones, st.l);
+    if constexpr (kSplit) {
+        st.l = TileF16::mfmaK32(lo, ones, st.l);
+    }
 
-#pragma unroll
-    for (int strip = 0; strip < L::kStrips; ++strip) {
-        float scale[8];
+    // eight columns (four: COLS) of this lane, from `byte` of the rows on
+    auto columns = [&](auto cols, int byte, const float (&scale)[8], int column) {
+        constexpr int COLS = decltype(cols)::value;
+        uint32_t codes[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            scale[j] = mx::scaleOf(s.vs[j][strip]);
+            const char *at = reinterpret_cast<const char *>(s.v) + (16 * (j / 4) + 4 * (j & 3) + g) * (HEAD / 2) + byte;
+            codes[j] = COLS == 8 ? *reinterpret_cast<const uint32_t *>(at) : *reinterpret_cast<const uint16_t *>(at);
         }
-        if (left < kStepTokens) { // a NaN there would pass through a probability of zero
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                scale[j] = 16 * (j / 4) + 4 * (j & 3) + g < left ? scale[j] : 0.0f;
-            }
-        }
-        constexpr int kFirst = L::kStripCols;
-        auto pair = [&](auto at, int word, int column) {
+        auto pair = [&](auto b) {
+            constexpr int B = decltype(b)::value;
             uint4 even, odd;
-            columnPair<decltype(at)::value, HEAD>(s, scale, word, even, odd);
-            st.o[column] = TileF16::mfmaK32(hi, even, st.o[column]);
-            st.o[column + 1] = TileF16::mfmaK32(hi, odd, st.o[column + 1]);
+            columnPair<B>(codes, scale, even, odd);
+            f32x4 &x = st.o[column + 2 * B], &y = st.o[column + 2 * B + 1];
+            x = TileF16::mfmaK32(hi, even, x);
+            y = TileF16::mfmaK32(hi, odd, y);
             if constexpr (kSplit) {
-                st.o[column] = TileF16::mfmaK32(lo, even, st.o[column]);
-                st.o[column + 1] = TileF16::mfmaK32(lo, odd, st.o[column + 1]);
+                x = TileF16::mfmaK32(lo, even, x);
+                y = TileF16::mfmaK32(lo, odd, y);
             }
             if constexpr (HEAD > 128) {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto word = [&](int w, int column, auto cols) {
-            pair(std::integral_constant<int, 0>{}, w, column);
-            pair(std::integral_constant<int, 1>{}, w, column + 2);
-            if constexpr (decltype(cols)::value == 8) {
-                pair(std::integral_constant<int, 2>{}, w, column + 4);
-                pair(std::integral_constant<int, 3>{}, w, column + 6);
+        pair(std::integral_constant<int, 0>{});
+        pair(std::integral_constant<int, 1>{});
+        if constexpr (COLS == 8) {
+            pair(std::integral_constant<int, 2>{});
+            pair(std::integral_constant<int, 3>{});
+        }
+    };
+#pragma unroll
+    for (int strip = 0; strip < L::kStrips; ++strip) {
+        const int byte = L::column(strip, c) / 2; // of a row; a scale covers 16
+        float scale[8];
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+            const uint4 w = reinterpret_cast<const uint4 *>(s.vs)[(4 * tile + g) * (HEAD / 32) + byte / 16];
+            scale[4 * tile] = mx::scaleOf(w.x);
+            scale[4 * tile + 1] = mx::scaleOf(w.y);
+            scale[4 * tile + 2] = mx::scaleOf(w.z);
+            scale[4 * tile + 3] = mx::scaleOf(w.w);
+        }
+        uint32_t bad = 0; // RUNS: bit j = the value of token j is not finite
+        if (masked) {     // a NaN there would pass through a probability of zero
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool seen = t0 + tokenOf(j) < tokens;
+                if constexpr (RUNS) { // by some row; which ones see it is settled below
+                    const bool finite = __float_as_uint(scale[j]) != 0x7f800000u;
+                    bad |= seen && !finite ? 1u << j : 0u;
+                    scale[j] = seen && finite ? scale[j] : 0.0f;
+                } else {
+                    scale[j] = seen ? scale[j] : 0.0f;
+                }
             }
-        };
-        if (strip == 0) {
-            word(0, 0, std::integral_constant<int, (kFirst < 8 ? 4 : 8)>{});
-            if constexpr (kFirst == 16) {
-                word(1, 8, std::integral_constant<int, 8>{});
-            }
+        }
+        if (strip == 1) {
+            columns(std::integral_constant<int, 4>{}, byte, scale, 8);
+        } else if constexpr (L::kStripCols == 4) {
+            columns(std::integral_constant<int, 4>{}, byte, scale, 0);
         } else {
-            word(1, 8, std::integral_constant<int, 4>{});
+            columns(std::integral_constant<int, 8>{}, byte, scale, 0);
+            if constexpr (L::kStripCols == 16) {
+                columns(std::integral_constant<int, 8>{}, byte + 4, scale, 8);
+            }
+        }
+        if constexpr (RUNS) {
+            if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) { // the columns of this strip, in the rows that see such a token
+                int first[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    first[i] = __shfl(rows.visible, 4 * g + i, 64) - t0; // the first token of the step that the row does not see
+                }
+#pragma unroll
+                for (int of = 0; of < 4; ++of) {
+                    const uint32_t theirs = __shfl(bad, 16 * of + c, 64);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int t = 16 * (j / 4) + 4 * (j & 3) + of;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if ((theirs >> j & 1) != 0 && t < first[i]) {
+#pragma unroll
+                                for (int e = 0; e < L::kCols; ++e) {
+                                    if ((e < L::kStripCols) == (strip == 0)) {
+                                        st.o[e][i] = NAN;
+                                    }
+                                }
+                            }
+                        }
+                    }
+                }
+            }
         }
     }
 }
 
-// The query heads of a chunk of sequence `seq`, in the order of the K elements; heads that the chunk does not have as zeros.
+// Row c of a segment: where its query and output vectors lie (in tokens and heads of q), and whether it is one.
+struct RowPlace {
+    bool exists;
+    int token, head;
+};
+template <bool RUNS>
+__device__ __forceinline__ RowPlace rowPlace(int group, int kv_head, int segment, int row, int first_token, int q_len) {
+    const int at = segment * kHeadsPerWave + row;
+    if constexpr (RUNS) {
+        const int token = at / group;
+        return {token < q_len, first_token + token, kv_head * group + at - token * group};
+    } else {
+        return {at < group, first_token, kv_head * group + at};
+    }
+}
+
+// A query vector, in the order of the K elements; a row that does not exist as zeros.
 template <typename T, int HEAD>
-__device__ __forceinline__ void loadQuery(const DecodeFp4Args &a, int seq, int kv_head, int chunk, int g, int c, uint4 (&q)[HEAD / 32]) {
+__device__ __forceinline__ void loadQuery(ArgsAgain a, const RowPlace &place, int g, uint4 (&q)[HEAD / 32]) {
     using L = Layout<HEAD>;
     using S = typename T::storage;
-    const int h = chunk * kHeadsPerWave + c;
-    const S *row = static_cast<const S *>(a.q) + seq * a.q_stride + (kv_head * a.group + min(h, a.group - 1)) * a.q_head_stride;
+    const S *row = static_cast<const S *>(a->q) + (place.exists ? place.token * a->q_stride + place.head * a->q_head_stride : 0);
+    const bool aligned = a->q_aligned;
 #pragma unroll
     for (int w = 0; w < L::kWords; ++w) {
         const S *at = row + L::element(w / 4, g) + 8 * (w & 3);
         uint4 x;
-        if (a.q_aligned) {
+        if (aligned) {
             x = *reinterpret_cast<const uint4 *>(at);
         } else {
             const uint16_t *e = reinterpret_cast<const uint16_t *>(at);
             x = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
         }
-        q[w] = h < a.group ? x : make_uint4(0, 0, 0, 0);
+        q[w] = place.exists ? x : make_uint4(0, 0, 0, 0);
     }
 }
 
@@ -481,38 +690,41 @@ __device__ __forceinline__ void storeColumns(typename T::storage *to, const floa
     }
 }
 
-// What the lanes hold of a run of steps: normalised outputs (`whole`), or a partial result at place `place`.
-template <typename T, int HEAD>
-__device__ __forceinline__ void finish(const DecodeFp4Args &a, const DecodeState<T, HEAD> &st, bool whole, int64_t place, int seq,
-                                       int kv_head, int chunk, int lane) {
+// What the lanes hold of a segment: normalised outputs (`whole`), or a partial result at place `place`.
+template <typename T, int HEAD, bool RUNS>
+__device__ __forceinline__ void finish(const DecodeState<T, HEAD> &st, const Rows &rows, bool whole, int64_t place, int kv_head,
+                                       int segment, int first_token, int q_len, int lane) {
     using L = Layout<HEAD>;
+    const ArgsAgain a = argsAgain();
     const int g = lane >> 4, c = lane & 15;
-    const float l = sumAcrossTokenGroups(st.l);
-    const int heads = min(a.group - chunk * kHeadsPerWave, kHeadsPerWave);
-    if (!whole && g == 0 && c < heads) {
-        a.part_ml[place * a.part_rows + c] = make_float2(st.m, l);
-    }
+    const int part_rows = a->part_rows;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int h = 4 * g + i;
-        const float f = whole ? 1.0f / __shfl(l, h, 64) : 1.0f;
-        if (h >= heads) {
+        const int r = 4 * g + i;
+        const float m = __shfl(st.m, r, 64);
+        const int visible = RUNS ? __shfl(rows.visible, r, 64) : 1;
+        const RowPlace at = rowPlace<RUNS>(a->group, kv_head, segment, r, first_token, q_len);
+        if (!at.exists || visible <= 0) {
             continue;
         }
+        const float f = whole ? 1.0f / st.l[i] : 1.0f;
         float x[L::kCols];
 #pragma unroll
         for (int e = 0; e < L::kCols; ++e) {
             x[e] = st.o[e][i] * f;
         }
         if (whole) {
-            auto *row = static_cast<typename T::storage *>(a.out) + seq * a.o_stride
-                      + (kv_head * a.group + chunk * kHeadsPerWave + h) * a.o_head_stride;
-            storeColumns<T, L::kStripCols>(row + L::column(0, c), x, a.out_aligned);
+            auto *row = static_cast<typename T::storage *>(a->out) + at.token * a->o_stride + at.head * a->o_head_stride;
+            const bool aligned = a->out_aligned;
+            storeColumns<T, L::kStripCols>(row + L::column(0, c), x, aligned);
             if constexpr (L::kStrips > 1) {
-                storeColumns<T, 4>(row + L::column(1, c), x + L::kStripCols, a.out_aligned);
+                storeColumns<T, 4>(row + L::column(1, c), x + L::kStripCols, aligned);
             }
         } else {
-            float *row = a.part_acc + (place * a.part_rows + h) * HEAD;
+            if (c == 0) {
+                a->part_ml[place * part_rows + r] = make_float2(m * rows.unit, st.l[i]);
+            }
+            float *row = a->part_acc + (place * part_rows + r) * HEAD;
 #pragma unroll
             for (int e = 0; e < L::kCols; e += 4) {
                 const int strip = e < L::kStripCols ? 0 : 1;
@@ -523,131 +735,236 @@ __device__ __forceinline__ void finish(const DecodeFp4Args &a, const DecodeState
     }
 }
 
-template <typename T, int HEAD, int GRAIN>
-__global__ void __launch_bounds__(kDecodeThreads, 2) decodeFp4Kernel(DecodeFp4Args a) {
+// Grid: KV heads x (runs / 4) x chunks of heads. Two neighbouring KV heads take turns on the dies: their scales share cache
+// lines, and a die that works on both at a time fetches them once.
+template <typename T, int HEAD, int GRAIN, bool RUNS>
+__global__ void __launch_bounds__(kDecodeThreads, Layout<HEAD>::kPerUnit)
+decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_type_, int32_t num_seqs, int32_t capacity, int32_t most_runs,
+                DecodeFp4Args a) {
+    using L = Layout<HEAD>;
+    constexpr int kStages = L::kStages;
+    __shared__ Step<HEAD> rings[kDecodeThreads / 64][kStages];
+    const IndexType index_type = static_cast<IndexType>(index_type_);
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int streams = a.num_kv_heads * a.head_chunks;
-    const int stream = blockIdx.x % streams;
-    const int run = static_cast<int>(blockIdx.x / streams) * (kDecodeThreads / 64) + wave;
-    const int kv_head = stream / a.head_chunks, chunk = stream % a.head_chunks;
+    auto work = [&](int seq) { return workOf<RUNS>(index_type, seq_lens, cu_seqlens_q, capacity, RUNS ? a.total_q_tokens : 0, RUNS ? a.group : 0, seq); };
 
-    const int64_t total = totalSteps(a, lane);
-    const int runs = runsFor(a, total);
+    // all steps, and with up to 64 sequences the work of each in a lane
+    Work mine{};
+    uint32_t total = 0, segments_of_all = 0;
+    for (int base = 0; base < num_seqs; base += 64) {
+        mine = base + lane < num_seqs ? work(base + lane) : Work{};
+        total += __builtin_amdgcn_readlane(waveInclusiveSum(static_cast<unsigned>(mine.all())), 63);
+        if constexpr (RUNS) {
+            segments_of_all += __builtin_amdgcn_readlane(waveInclusiveSum(mine.steps > 0 ? mine.segments : 0), 63);
+        }
+    }
+    const bool paired = (gridDim.x & 1) == 0 && (gridDim.y & 1) == 0;
+    const int kv_head = paired ? (blockIdx.x & ~1u) | (blockIdx.y & 1) : blockIdx.x;
+    const uint32_t run = 4 * (paired ? (blockIdx.y & ~1u) | (blockIdx.x & 1) : blockIdx.y) + wave;
+    const int chunk = blockIdx.z;
+    const uint32_t runs = runsFor(most_runs, total);
+    if (RUNS && blockIdx.x + blockIdx.y == 0 && threadIdx.x == 0 && a.num_segments != nullptr) {
+        *a.num_segments = segments_of_all;
+    }
     if (run >= runs) {
         return;
     }
-    int64_t at = runStart(total, runs, run);
-    const int64_t end = runStart(total, runs, run + 1);
+    const Cut cut(total, runs);
+    uint32_t at = cut.start(run);
+    const uint32_t end = cut.start(run + 1);
 
-    const float slope = a.alibi_slopes != nullptr && chunk * kHeadsPerWave + c < a.group
-                          ? a.alibi_slopes[kv_head * a.group + chunk * kHeadsPerWave + c] * kLog2e : 0.0f;
-    Pages<HEAD, GRAIN> pages{a, lane, g, c, kv_head};
+    auto &ring = rings[wave];
+    Pages<HEAD, GRAIN> pages(a, lane, kv_head);
     DecodeState<T, HEAD> st;
+    Rows rows;
+    rows.plain = a.alibi_slopes == nullptr && a.scale_log2 > 0.0f;
+    rows.scale_log2 = a.scale_log2;
+    rows.unit = rows.plain ? a.scale_log2 : 1.0f;
+    rows.lazy = kLazyLog2 / rows.unit;
+    rows.visible = rows.least = 0;
 
-    int64_t before = 0; // steps of the sequences in front of the 64 at hand
-    for (int base = 0; base < a.num_seqs && at < end; base += 64) {
-        const int tokens_of = base + lane < a.num_seqs ? sequenceTokens(a, base + lane) : 0;
-        const int sum = waveInclusiveSum(stepsOf(tokens_of));
-        const int all = __builtin_amdgcn_readlane(sum, 63);
+    uint32_t before = 0, segments_before = 0; // of the sequences in front of the 64 at hand
+    for (int base = 0; base < num_seqs && at < end; base += 64) {
+        if (num_seqs > 64) {
+            mine = base + lane < num_seqs ? work(base + lane) : Work{};
+        }
+        const uint32_t sum = waveInclusiveSum(static_cast<unsigned>(mine.all()));
+        const uint32_t segment_sum = RUNS ? waveInclusiveSum(static_cast<unsigned>(mine.steps > 0 ? mine.segments : 0)) : 0;
+        const uint32_t all = __builtin_amdgcn_readlane(sum, 63);
         while (at < end && at < before + all) {
             // the first sequence that ends behind `at`
             const int in = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before + sum > at));
-            const int tokens = __builtin_amdgcn_readlane(tokens_of, in);
+            const int tokens = __builtin_amdgcn_readlane(mine.tokens, in);
             const int steps = stepsOf(tokens);
-            const int64_t start = before + __builtin_amdgcn_readlane(sum, in) - steps;
             const int seq = base + in;
+            int first_token = seq, q_len = 1, segment = chunk, history = 0;
+            uint32_t start = before + __builtin_amdgcn_readlane(sum, in) - steps;
+            int id = seq;
+            if constexpr (RUNS) {
+                first_token = __builtin_amdgcn_readlane(mine.q_start, in);
+                q_len = __builtin_amdgcn_readlane(mine.q_len, in);
+                history = __builtin_amdgcn_readlane(mine.history, in);
+                const int segments = __builtin_amdgcn_readlane(mine.segments, in);
+                start -= (segments - 1) * steps;
+                segment = (at - start) / steps;
+                start += segment * steps;
+                id = segments_before + __builtin_amdgcn_readlane(segment_sum, in) - segments + segment;
+            }
             const int from = static_cast<int>(at - start);
-            const int to = static_cast<int>(end - start < steps ? end - start : steps);
+            const int to = static_cast<int>(end - start < static_cast<uint32_t>(steps) ? end - start : steps);
 
-            pages.begin(seq, tokens, from);
-            Step<HEAD> ahead[2];
-            pages.load(ahead[0]);
-            loadQuery<T, HEAD>(a, seq, kv_head, chunk, g, c, st.q);
+            pages.begin(seq * argsAgain()->block_table_stride, tokens, from);
+#pragma unroll
+            for (int i = 0; i < kStages; ++i) {
+                if (from + i < to) {
+                    pages.load(ring[i]);
+                }
+            }
+            {
+                const ArgsAgain again = argsAgain();
+                const RowPlace place = rowPlace<RUNS>(again->group, kv_head, segment, c, first_token, q_len);
+                loadQuery<T, HEAD>(again, place, g, st.q);
+                rows.slope_log2 = !rows.plain && again->alibi_slopes != nullptr && place.exists ? again->alibi_slopes[place.head] * kLog2e : 0.0f;
+                if constexpr (RUNS) {
+                    const int sees = history + (place.token - first_token) + 1;
+                    rows.visible = !place.exists || sees < 0 ? 0 : (sees > tokens ? tokens : sees);
+                    rows.least = __builtin_amdgcn_readfirstlane(-waveMaxInt(-(place.exists ? rows.visible : 0x7fffffff)));
+                }
+            }
             st.m = -INFINITY;
-            st.l = 0.0f;
+            st.shift = 0.0f;
+            st.l = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int e = 0; e < HEAD / 16; ++e) {
                 st.o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
-            auto compute = [&](const Step<HEAD> &s, int step) {
-                const int left = tokens - step * kStepTokens;
-                // (1 - left: of the step's first token from the last one)
-                computeStep<T, HEAD>(a, s, st, g, left, slope, static_cast<float>(1 - left));
-            };
-            for (int step = from; step < to; step += 2) {
-                if (step + 1 < to) {
-                    pages.load(ahead[1]);
+            int stage = 0;
+            for (int step = from; step < to; ++step) {
+                // the loads of this step are done; those of the steps behind it, up to kStages - 1, may be under way
+                const int behind = to - 1 - step;
+                if (behind >= kStages - 1) {
+                    waitLoads<(kStages - 1) * L::kLoads>();
+                } else if (kStages > 3 && behind >= 2) {
+                    waitLoads<(kStages > 3 ? 2 : 0) * L::kLoads>();
+                } else if (kStages > 2 && behind >= 1) {
+                    waitLoads<(kStages > 2 ? 1 : 0) * L::kLoads>();
+                } else {
+                    waitLoads<0>();
                 }
-                compute(ahead[0], step);
-                if (step + 1 < to) {
-                    if (step + 2 < to) {
-                        pages.load(ahead[0]);
-                    }
-                    compute(ahead[1], step + 1);
+                computeStep<T, HEAD, RUNS>(ring[stage], st, rows, lane, step * kStepTokens, tokens);
+                if (step + kStages < to) {
+                    pages.load(ring[stage]);
+                }
+                stage = stage + 1 < kStages ? stage + 1 : 0;
+            }
+            const bool whole = from == 0 && to == steps;
+            if (from == 0) {
+                const ArgsAgain again = argsAgain();
+                if (again->segments != nullptr && kv_head + chunk == 0 && lane == 0) { // the same in every stream
+                    again->segments[id] = make_int4(run, cut.runOf(start + steps - 1), seq, segment);
                 }
             }
-            const int64_t place = (static_cast<int64_t>(stream) * a.runs + run) * 2 + (from == 0 ? 1 : 0);
-            finish<T, HEAD>(a, st, from == 0 && to == steps, place, seq, kv_head, chunk, lane);
+            const int64_t place = (static_cast<int64_t>(kv_head * static_cast<int>(gridDim.z) + chunk) * most_runs + run) * 2 + (from == 0 ? 1 : 0);
+            finish<T, HEAD, RUNS>(st, rows, whole, place, kv_head, segment, first_token, q_len, lane);
             at = start + to;
         }
         before += all;
+        segments_before += RUNS ? __builtin_amdgcn_readlane(segment_sum, 63) : 0;
     }
 }
 
-// One wavefront per (sequence, query head): the parts of a sequence that lies in more than one run, joined in their order.
-template <typename T, int HEAD>
-__global__ void __launch_bounds__(64) mergeFp4Kernel(DecodeFp4Args a) {
-    const int lane = threadIdx.x;
-    const int seq = blockIdx.x / a.num_heads, head = blockIdx.x % a.num_heads;
-    const int steps = stepsOf(sequenceTokens(a, seq));
-    if (steps == 0) {
-        return;
-    }
-    int64_t total = 0, start = 0;
-    for (int base = 0; base < a.num_seqs; base += 64) {
-        const int n = base + lane < a.num_seqs ? stepsOf(sequenceTokens(a, base + lane)) : 0;
-        total += __builtin_amdgcn_readlane(waveInclusiveSum(n), 63);
-        start += __builtin_amdgcn_readlane(waveInclusiveSum(base + lane < seq ? n : 0), 63);
-    }
-    const int runs = runsFor(a, total);
-    const int first = runOf(total, runs, start), last = runOf(total, runs, start + steps - 1);
-    if (first == last) {
-        return; // whole: written already
-    }
-    const int kv_head = head / a.group, in_group = head % a.group;
-    const int stream = kv_head * a.head_chunks + in_group / kHeadsPerWave;
-    const int row = in_group % kHeadsPerWave;
-    // a part is at place 1 where the sequence begins in that run, else at 0
-    auto placeOf = [&](int run) {
-        return ((static_cast<int64_t>(stream) * a.runs + run) * 2 + (run == first ? 1 : 0)) * a.part_rows + row;
-    };
-    float m = -INFINITY;
-    for (int run = first + lane; run <= last; run += 64) {
-        m = maxOf(m, a.part_ml[placeOf(run)].x);
-    }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        m = maxOf(m, __shfl_xor(m, off, 64));
-    }
-    constexpr int kPer = HEAD / 64;
-    float l = 0.0f, x[kPer] = {};
-#pragma unroll 4
-    for (int run = first; run <= last; ++run) {
-        const int64_t place = placeOf(run);
-        const float2 ml = a.part_ml[place];
-        const float f = fastExp2(ml.x - m);
-        l += ml.y * f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            x[i] += a.part_acc[place * HEAD + 64 * i + lane] * f;
+// The parts of a segment that lies in more than one run, joined: a workgroup per (segment, row, stream). A quarter of the
+// HEAD columns is a lane's four, so that 64 / (HEAD / 4) groups of lanes (of WAVES wavefronts) share the parts, each in the
+// order of the runs; the groups are joined in LDS, in their order.
+template <typename T, int HEAD, bool RUNS, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) mergeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_type_, int32_t num_seqs,
+                                                             int32_t capacity, int32_t most_runs, DecodeFp4Args a) {
+    constexpr int kLanes = HEAD / 4, kGroups = 64 * WAVES / kLanes; // (head 192: 48 lanes, some groups have lanes of two wavefronts)
+    const int row = blockIdx.x % a.part_rows, id = blockIdx.x / a.part_rows;
+    const int kv_head = blockIdx.y, chunk = blockIdx.z;
+    const int group = threadIdx.x / kLanes, column = 4 * (threadIdx.x % kLanes);
+    if constexpr (RUNS) {
+        if (id >= *a.num_segments) {
+            return;
         }
     }
-    auto *to = static_cast<typename T::storage *>(a.out) + seq * a.o_stride + head * a.o_head_stride;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        to[64 * i + lane] = T::Base::fromFloat(x[i] * (1.0f / l));
+    const int4 segment = a.segments[id];
+    const IndexType index_type = static_cast<IndexType>(index_type_);
+    const Work w = workOf<RUNS>(index_type, seq_lens, cu_seqlens_q, capacity, RUNS ? a.total_q_tokens : 0, RUNS ? a.group : 0, RUNS ? segment.z : id);
+    const RowPlace at = rowPlace<RUNS>(a.group, kv_head, RUNS ? segment.w : chunk, row, RUNS ? w.q_start : id, w.q_len);
+    if (w.steps == 0 || !at.exists || (RUNS && w.history + (at.token - w.q_start) + 1 <= 0)) {
+        return; // (without tokens nobody has written the segment)
     }
+    const int first = segment.x, parts = segment.y - segment.x + 1;
+    if (parts <= 1) {
+        return; // whole: written already
+    }
+    // a part is at place 1 where the segment begins in that run, else at 0
+    const int64_t stream = static_cast<int64_t>(kv_head * static_cast<int>(gridDim.z) + chunk) * most_runs;
+    auto placeOf = [&](int part) { return ((stream + first + part) * 2 + (part == 0 ? 1 : 0)) * a.part_rows + row; };
+    float m = -INFINITY, l = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int kAhead = 4;
+    if (group < kGroups) {
+        for (int part = group; part < parts; part += kAhead * kGroups) {
+            float2 ml[kAhead];
+            float4 v[kAhead];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) { // (beyond the last: it again, without weight)
+                const int64_t place = placeOf(min(part + i * kGroups, parts - 1));
+                ml[i] = a.part_ml[place];
+                v[i] = *reinterpret_cast<const float4 *>(a.part_acc + place * HEAD + column);
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) {
+                if (part + i * kGroups < parts) {
+                    const float top = maxOf(m, ml[i].x);
+                    // (no weight at all so far, on either side: m = -inf, l = 0 and zeros)
+                    const float keep = m == top ? 1.0f : fastExp2(m - top), add = ml[i].x == top ? 1.0f : fastExp2(ml[i].x - top);
+                    m = top;
+                    l = l * keep + ml[i].y * add;
+                    x.x = x.x * keep + v[i].x * add;
+                    x.y = x.y * keep + v[i].y * add;
+                    x.z = x.z * keep + v[i].z * add;
+                    x.w = x.w * keep + v[i].w * add;
+                }
+            }
+        }
+    }
+    __shared__ float2 their_ml[kGroups];
+    __shared__ float4 theirs[kGroups][kLanes];
+    if (group < kGroups) {
+        theirs[group][threadIdx.x % kLanes] = x;
+        if (column == 0) {
+            their_ml[group] = make_float2(m, l);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= kLanes) {
+        return;
+    }
+    m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+        m = maxOf(m, their_ml[i].x);
+    }
+    l = 0.0f;
+    x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kGroups; ++i) {
+        const float2 ml = their_ml[i];
+        const float f = ml.x == m ? 1.0f : fastExp2(ml.x - m);
+        const float4 v = theirs[i][threadIdx.x];
+        l += ml.y * f;
+        x.x += v.x * f;
+        x.y += v.y * f;
+        x.z += v.z * f;
+        x.w += v.w * f;
+    }
+    const float f = 1.0f / l;
+    const float y[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
+    storeColumns<T, 4>(static_cast<typename T::storage *>(a.out) + at.token * a.o_stride + at.head * a.o_head_stride + column, y, a.out_aligned);
 }
 
 } // namespace op::paged_attention_fp4::amd

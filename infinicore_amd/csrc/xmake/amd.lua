@@ -92,8 +92,8 @@ target("infiniop-amd")
     -- the scatter kernel gets its first 14 argument words in scalar registers at wavefront start
     add_files("../src/infiniop/ops/paged_caching/amd/*.hip", {cxflags = {"-mllvm", "-amdgpu-kernarg-preload-count=14"}})
     -- the attention kernels keep their matrix-instruction accumulators in ordinary vector registers
-    add_files("../src/infiniop/ops/paged_attention_fp4/amd/*.hip", {cxflags = {"-mllvm", "-amdgpu-mfma-vgpr-form=1"}})
-    add_files("../src/infiniop/ops/paged_attention_prefill_fp4/amd/*.hip", {cxflags = {"-mllvm", "-amdgpu-mfma-vgpr-form=1"}})
+    add_files("../src/infiniop/ops/paged_attention_fp4/amd/*.hip", {cxflags = {"-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-amdgpu-kernarg-preload-count=8"}})
+    add_files("../src/infiniop/ops/paged_attention_prefill_fp4/amd/*.hip", {cxflags = {"-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-amdgpu-kernarg-preload-count=8"}})
     add_files("../src/infiniop/ops/paged_attention_prefill/amd/*.hip", {cxflags = {"-mllvm", "-amdgpu-mfma-vgpr-form=1"}})
     -- decode also gets the first five argument words of its work-equalising kernels in scalar registers at wavefront start
     add_files("../src/infiniop/ops/paged_attention/amd/*.hip",
