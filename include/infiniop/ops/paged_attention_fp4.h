@@ -7,7 +7,7 @@
  *   q             [num_seqs, num_heads, head_size]   same dtype
  *   k_codes       [num_blocks, num_kv_heads, block_size, head_size / 2]   U8, strides of dims 0-2 multiples of 16
  *   v_codes       like k_codes
- *   k_scales      [num_blocks, num_kv_heads, block_size, head_size / 32]  U8, any strides on dims 0-2
+ *   k_scales      [num_blocks, num_kv_heads, block_size, head_size / 32]  U8, strides of dims 0-2 multiples of 4 (head_size 64, 192: 2)
  *   v_scales      like k_scales
  *   block_tables  [num_seqs or more, max_blocks_per_seq]  I64 | I32 | U32
  *   seq_lens      [num_seqs]                              same index dtype; tokens of each sequence, the current one included
@@ -49,7 +49,7 @@ __INFINI_C __export infiniStatus_t infiniopGetPagedAttentionFp4WorkspaceSize(
     size_t *size);
 
 /* Enqueues on `stream`, allocates nothing and waits for nothing. BAD_PARAM where the calling thread's current device is not
- * the descriptor's, or where codes do not begin at a multiple of 16 bytes. */
+ * the descriptor's, or where codes do not begin at a multiple of 16 bytes or scales of 4 (2). */
 __INFINI_C __export infiniStatus_t infiniopPagedAttentionFp4(
     infiniopPagedAttentionFp4Descriptor_t desc,
     void *workspace,

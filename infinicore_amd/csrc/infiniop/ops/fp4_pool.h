@@ -64,15 +64,16 @@ struct PoolInfo {
         return info;
     }
 
-    // Whether every row of the codes begins at a multiple of `bytes` from the base.
-    bool codeRowsAligned(size_t bytes) const {
+    // Whether every row of the codes (scales) begins at a multiple of `bytes` from the base.
+    bool codeRowsAligned(size_t bytes) const { return rowsAligned(k_codes, bytes) && rowsAligned(v_codes, bytes); }
+    bool scaleRowsAligned(size_t bytes) const { return rowsAligned(k_scales, bytes) && rowsAligned(v_scales, bytes); }
+
+    bool rowsAligned(const PoolStrides &s, size_t bytes) const {
         const size_t extent[3] = {num_blocks, num_kv_heads, block_size};
-        for (const PoolStrides &s : {k_codes, v_codes}) {
-            const ptrdiff_t stride[3] = {s.block, s.head, s.row};
-            for (int i = 0; i < 3; ++i) {
-                if (extent[i] > 1 && static_cast<size_t>(stride[i]) % bytes != 0) {
-                    return false;
-                }
+        const ptrdiff_t stride[3] = {s.block, s.head, s.row};
+        for (int i = 0; i < 3; ++i) {
+            if (extent[i] > 1 && static_cast<size_t>(stride[i]) % bytes != 0) {
+                return false;
             }
         }
         return true;

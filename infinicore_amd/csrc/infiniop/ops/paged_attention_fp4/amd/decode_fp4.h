@@ -21,10 +21,14 @@
 // in fp16, where every written value is exact and the probabilities keep eleven bits (as bf16 they would add an error as large
 // as the output's own rounding). For fp16 outputs the probabilities go in as two terms for the same reason.
 //
-// Work is dealt by steps: the steps of all sequences, one after the other, are cut into as many equal runs as there are
-// wavefronts for a KV head. A run may hold the end of one sequence, whole ones, and the start of another; whole sequences are
-// normalised and written at once, the others leave accumulators, reference points and denominators, which the merge kernel
-// joins in the order of the runs.
+// Work is dealt in one of two ways (wholeSequences in decode_fp4_launch.h has the times on both sides):
+//   * whole: a workgroup of eight wavefronts for a sequence and KV head, joined in LDS;
+//   * by runs: the steps of all sequences, one after the other, are cut into as many equal runs as there are wavefronts for a KV
+//     head. A run may hold the end of one sequence, whole ones, and the start of another; whole sequences are normalised and
+//     written at once, the others leave accumulators, reference points and denominators, which the merge kernel joins in the
+//     order of the runs.
+// RUNS (runs of a few query tokens per sequence, for prefill): rows are (query token, head) pairs, 16 to a segment, each with
+// the tokens that it sees.
 #ifndef INFINICORE_AMD_PA_DECODE_FP4_H
 #define INFINICORE_AMD_PA_DECODE_FP4_H
 
@@ -51,6 +55,7 @@ namespace mx = device::amd::mx;
 
 constexpr int kStepTokens = 32;
 constexpr int kDecodeThreads = 256;  // four wavefronts that share nothing but the launch
+constexpr int kWholeThreads = 512;
 constexpr int kLeastSteps = 1;       // of a run
 constexpr float kLazyLog2 = 8.0f;    // how far (in powers of two) a maximum may outgrow its reference point
 
@@ -211,37 +216,43 @@ struct Layout {
     static __device__ __forceinline__ int kSlot(int row, int chunk) {
         return row * kChunks + (chunk ^ (((row & 15) * kChunks / 16) & (HEAD == 192 ? 1 : kChunks - 1)));
     }
-    // Load instructions of a step: codes (of K, of V), scales of K, of V.
-    static constexpr int kCodeLoads = HEAD / 64, kKScaleLoads = 2 * kPieces, kVScaleLoads = HEAD / 64;
-    static constexpr int kLoads = 2 * kCodeLoads + kKScaleLoads + kVScaleLoads;
+    // Scales are loaded in units of four, where a row has a multiple of four, else of two.
+    static constexpr int kScaleUnit = HEAD % 128 == 0 ? 4 : 2, kScaleUnits = HEAD / 32 / kScaleUnit;
+    // Load instructions of a step: codes (of K, of V), scales (one unit of 32 rows of K and of V each)
+    static constexpr int kCodeLoads = HEAD / 64;
+    static constexpr int kLoads = 2 * kCodeLoads + kScaleUnits;
     // Workgroups (of four wavefronts) that share a compute unit, and the steps in flight or at hand that its 160 KiB of LDS
     // then hold for each wavefront.
-    static constexpr int kPerUnit = HEAD == 64 ? 3 : (HEAD == 128 ? 3 : 2);
-    static constexpr int kStages = HEAD == 64 ? 4 : 2;
+    static constexpr int kPerUnit = HEAD == 64 ? 3 : 2;
+    static constexpr int kStages = HEAD <= 128 ? 3 : 2;
+    // The same for workgroups of eight that have a sequence to themselves.
+    static constexpr int kWholePerUnit = HEAD == 64 ? 2 : 1;
+    static constexpr int kWholeStages = HEAD == 64 ? 4 : (HEAD == 128 ? 3 : 2);
 };
 
-// One step in LDS. A scale has a dword of its own: K [tile][piece][lane], V [tile][group g][scale of the row][i].
+// One step in LDS. A unit of scales has a dword: [unit][32 rows of K, 32 of V]; row 16 tile + c of K is that of lane c, row
+// 16 tile + 4 g + i of V is token 4 i + g of the tile, so that a lane's four are neighbours.
 template <int HEAD>
 struct Step {
     using L = Layout<HEAD>;
     uint4 k[64 * L::kCodeLoads], v[64 * L::kCodeLoads];
-    uint32_t ks[64 * L::kKScaleLoads], vs[64 * L::kVScaleLoads];
+    uint32_t scales[L::kScaleUnits][64];
 };
 
-// From global memory straight into LDS, as loadLane16ToLds does for 16 bytes: a byte of each lane, widened to a dword. Lane i
-// writes lds_base + 4 i.
+// From global memory straight into LDS, as loadLane16ToLds does for 16 bytes: a unit of scales of each lane, in a dword. Lane i
+// writes lds_base + 4 i. (Through the caches, unlike the codes: the scales of two KV heads share lines.)
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ uint32_t ldsAddress(const void *p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const void *)p));
 }
-__device__ __forceinline__ void loadByteToLds(const char *uniform_base, uint32_t lane_offset, uint32_t *lds_base) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, %1 nt"
-                 :: "v"(lane_offset), "s"(uniform_base), "s"(ldsAddress(lds_base)) : "memory", "m0");
-}
-__device__ __forceinline__ void loadByteToLds(const char *lane_pointer, uint32_t *lds_base) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off nt"
-                 :: "v"(lane_pointer), "s"(ldsAddress(lds_base)) : "memory", "m0");
+template <int BYTES>
+__device__ __forceinline__ void loadScalesToLds(const char *lane_pointer, uint32_t *lds_base) {
+    if constexpr (BYTES == 4) {
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" :: "v"(lane_pointer), "s"(ldsAddress(lds_base)) : "memory", "m0");
+    } else {
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ushort %0, off" :: "v"(lane_pointer), "s"(ldsAddress(lds_base)) : "memory", "m0");
+    }
 }
 #pragma clang diagnostic pop
 // All but the last LEFT of this wavefront's vector memory operations are done.
@@ -372,13 +383,7 @@ struct Pages {
             __device__ __forceinline__ void operator()(const char *base, uint32_t offset) const { loadLane16ToLds<true>(base, offset, to); }
             __device__ __forceinline__ void operator()(const char *p) const { loadLane16ToLds<true>(p, to); }
         };
-        struct Byte {
-            uint32_t *to;
-            __device__ __forceinline__ void operator()(const char *base, uint32_t offset) const { loadByteToLds(base, offset, to); }
-            __device__ __forceinline__ void operator()(const char *p) const { loadByteToLds(p, to); }
-        };
-        constexpr int C = L::kChunks, kScales = HEAD / 32;
-        const int g = lane >> 4, c = lane & 15;
+        constexpr int C = L::kChunks;
         waitLdsReads();
         auto codes = [&](auto j) {
             constexpr int J = decltype(j)::value;
@@ -386,20 +391,25 @@ struct Pages {
             const int r = (64 * J + lane) / C, at = (64 * J + lane) % C;
             each<first, last>(&DecodeFp4Args::k_codes, k_code_row, kc, r, 16 * (L::kSlot(r, at) - r * C), Chunk{to.k + 64 * J}); // (exchanged twice is back)
             each<first, last>(&DecodeFp4Args::v_codes, v_code_row, vc, r, 16 * at, Chunk{to.v + 64 * J});
-            // V scales: 4 kScales entries for each of the eight (tile, group) pairs
-            const int e = 64 * J + lane, pair = e / (4 * kScales), scale = e % (4 * kScales) / 4, i = e & 3;
-            constexpr int first_tile = 64 * J / (16 * kScales), last_tile = (64 * J + 63) / (16 * kScales);
-            each<16 * first_tile, 16 * last_tile + 15>(&DecodeFp4Args::v_scales, v_scale_row, vs, 16 * (pair >> 2) + 4 * i + (pair & 3), scale, Byte{to.vs + 64 * J});
         };
         codes(std::integral_constant<int, 0>{});
         if constexpr (L::kCodeLoads > 1) { codes(std::integral_constant<int, 1>{}); }
         if constexpr (L::kCodeLoads > 2) { codes(std::integral_constant<int, 2>{}); }
         if constexpr (L::kCodeLoads > 3) { codes(std::integral_constant<int, 3>{}); }
-        const int m = 4 * (c & 3) + (c >> 2);
+        const int r = lane & 31, t = (r & 16) + 4 * (r & 3) + ((r >> 2) & 3); // (for K and V alike: see Step and Layout)
+        const char *from;
+        if constexpr (GRAIN > 1) {
+            const char *k_row = pick<0, kUnits - 1>(ks, t / GRAIN) + (t % GRAIN) * k_scale_row;
+            const char *v_row = pick<0, kUnits - 1>(vs, t / GRAIN) + (t % GRAIN) * v_scale_row;
+            from = lane < 32 ? k_row : v_row;
+        } else {
+            const ArgsAgain a = argsAgain();
+            const int id = __shfl(ids, t, 64), in = __shfl(row, t, 64);
+            from = lane < 32 ? rowOf(a->k_scales, id, in) : rowOf(a->v_scales, id, in);
+        }
 #pragma unroll
-        for (int p = 0; p < L::kPieces; ++p) {
-            each<0, 15>(&DecodeFp4Args::k_scales, k_scale_row, ks, m, L::element(p, g) / 32, Byte{to.ks + 64 * p});
-            each<16, 31>(&DecodeFp4Args::k_scales, k_scale_row, ks, 16 + m, L::element(p, g) / 32, Byte{to.ks + 64 * (L::kPieces + p)});
+        for (int u = 0; u < L::kScaleUnits; ++u) {
+            loadScalesToLds<L::kScaleUnit>(from + u * L::kScaleUnit, to.scales[u]);
         }
         token += kStepTokens;
         if constexpr (GRAIN == 1) {
@@ -438,6 +448,21 @@ __device__ __forceinline__ void columnPair(const uint32_t (&codes)[8], const flo
     odd = make_uint4(high(w[0], w[1]), high(w[2], w[3]), high(w[4], w[5]), high(w[6], w[7]));
 }
 
+// Scale `byte` of a unit, as the conversions take it: rotated to where a float has its exponent. (What lies in the sign and
+// the significand does not count; held against the same scales with zeros there on the device.)
+__device__ __forceinline__ float scaleIn(uint32_t unit, int byte) {
+    return __uint_as_float(__builtin_amdgcn_alignbit(unit, unit, 8 * byte + 9));
+}
+
+// f(0), f(1), .., f(N - 1), each with its number as a constant.
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void eachIndex(const F &f) {
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        eachIndex<N, I + 1>(f);
+    }
+}
+
 // What is the same for every step of a segment.
 struct Rows {
     float scale_log2, slope_log2; // slope: of row c
@@ -445,6 +470,12 @@ struct Rows {
     bool plain;                   // no ALiBi and a positive scale: maxima are kept in units of the raw product
     int visible;                  // tokens that row c sees
     int least;                    // and the row of the segment that sees the fewest
+
+    __device__ __forceinline__ Rows(const DecodeFp4Args &a)
+        : scale_log2(a.scale_log2), slope_log2(0.0f), plain(a.alibi_slopes == nullptr && a.scale_log2 > 0.0f), visible(0), least(0) {
+        unit = plain ? scale_log2 : 1.0f;
+        lazy = kLazyLog2 / unit;
+    }
 };
 
 // One step, from token t0 on. Tokens that a row does not see, and those behind the sequence, have no part in it, whatever their
@@ -453,33 +484,97 @@ template <typename T, int HEAD, bool RUNS>
 __device__ __forceinline__ void computeStep(const Step<HEAD> &s, DecodeState<T, HEAD> &st, const Rows &rows, int lane, int t0, int tokens) {
     using L = Layout<HEAD>;
     constexpr bool kSplit = T::kSplitProbabilities == false; // fp16 outputs: two terms (see the top)
+    constexpr int kPairs = HEAD / 32;                         // of columns a lane has
     const int g = lane >> 4, c = lane & 15, k_row = 4 * (c & 3) + (c >> 2);
+    auto tokenOf = [&](int j) { return 16 * (j / 4) + 4 * (j & 3) + g; }; // of the step
+    const bool masked = t0 + kStepTokens > (RUNS ? rows.least : tokens);
+
+    uint32_t codes[L::kVWords][8];
+    float scale[L::kStrips][8];
+    uint32_t bad[L::kStrips]; // RUNS: bit j = the value of token j is not finite
+#pragma unroll
+    for (int strip = 0; strip < L::kStrips; ++strip) {
+        const int byte = L::column(strip, c) / 2; // of a row; a scale covers 16
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const char *at = reinterpret_cast<const char *>(s.v) + tokenOf(j) * (HEAD / 2) + byte;
+            if (strip == 1 || L::kStripCols == 4) {
+                codes[strip][j] = *reinterpret_cast<const uint16_t *>(at);
+            } else if constexpr (L::kStripCols == 8) {
+                codes[0][j] = *reinterpret_cast<const uint32_t *>(at);
+            } else {
+                const uint2 w = *reinterpret_cast<const uint2 *>(at);
+                codes[0][j] = w.x;
+                codes[L::kVWords - 1][j] = w.y;
+            }
+        }
+        const int group = byte / 16;
+#pragma unroll
+        for (int tile = 0; tile < 2; ++tile) {
+            const uint4 w = *reinterpret_cast<const uint4 *>(&s.scales[group / L::kScaleUnit][32 + 16 * tile + 4 * g]);
+            scale[strip][4 * tile] = scaleIn(w.x, group % L::kScaleUnit);
+            scale[strip][4 * tile + 1] = scaleIn(w.y, group % L::kScaleUnit);
+            scale[strip][4 * tile + 2] = scaleIn(w.z, group % L::kScaleUnit);
+            scale[strip][4 * tile + 3] = scaleIn(w.w, group % L::kScaleUnit);
+        }
+        bad[strip] = 0;
+    }
+    uint4 kw[2][L::kPieces];
+    float k_scale[2][L::kPieces];
+#pragma unroll
+    for (int tile = 0; tile < 2; ++tile) {
+#pragma unroll
+        for (int p = 0; p < L::kPieces; ++p) {
+            const int group = L::element(p, g) / 32;
+            k_scale[tile][p] = scaleIn(s.scales[group / L::kScaleUnit][16 * tile + c], group % L::kScaleUnit);
+            const uint4 *row = s.k + 16 * tile * L::kChunks;
+            if (L::pieceWhole(p)) {
+                kw[tile][p] = row[L::kSlot(k_row, 4 * p + g)];
+            } else {
+                const uint2 w = reinterpret_cast<const uint2 *>(row + L::kSlot(k_row, 4 * p + (g >> 1)))[g & 1];
+                kw[tile][p] = make_uint4(w.x, w.y, 0, 0);
+            }
+        }
+    }
+    if (masked) { // a NaN there would pass through a probability of zero
+#pragma unroll
+        for (int strip = 0; strip < L::kStrips; ++strip) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool seen = t0 + tokenOf(j) < tokens;
+                if constexpr (RUNS) { // by some row; which ones see it is settled below
+                    const bool finite = (__float_as_uint(scale[strip][j]) & 0x7f800000u) != 0x7f800000u;
+                    bad[strip] |= seen && !finite ? 1u << j : 0u;
+                    scale[strip][j] = seen && finite ? scale[strip][j] : 0.0f;
+                } else {
+                    scale[strip][j] = seen ? scale[strip][j] : 0.0f;
+                }
+            }
+        }
+    }
+    // operands of columns 2 x and 2 x + 1
+    auto operands = [&](auto x, uint4 &even, uint4 &odd) {
+        constexpr int X = decltype(x)::value;
+        constexpr int strip = 2 * X < L::kStripCols ? 0 : 1;
+        constexpr int word = L::kStrips > 1 ? strip : X / 4, byte = L::kStrips > 1 && strip == 1 ? X - L::kStripCols / 2 : X % 4;
+        columnPair<byte>(codes[word], scale[strip], even, odd);
+    };
     f32x4 score[2];
 #pragma unroll
     for (int tile = 0; tile < 2; ++tile) {
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int p = 0; p < L::kPieces; ++p) {
-            const float scale = mx::scaleOf(s.ks[64 * (L::kPieces * tile + p) + lane]);
-            const uint4 *row = s.k + 16 * tile * L::kChunks;
-            {
-                if (L::pieceWhole(p)) {
-                    const uint4 w = row[L::kSlot(k_row, 4 * p + g)];
-                    x = T::mfmaK32(toQueryType<T>(w.x, scale), st.q[4 * p], x);
-                    x = T::mfmaK32(toQueryType<T>(w.y, scale), st.q[4 * p + 1], x);
-                    x = T::mfmaK32(toQueryType<T>(w.z, scale), st.q[4 * p + (L::kWords > 2 ? 2 : 0)], x);
-                    x = T::mfmaK32(toQueryType<T>(w.w, scale), st.q[4 * p + (L::kWords > 2 ? 3 : 0)], x);
-                } else {
-                    const uint2 w = reinterpret_cast<const uint2 *>(row + L::kSlot(k_row, 4 * p + (g >> 1)))[g & 1];
-                    x = T::mfmaK32(toQueryType<T>(w.x, scale), st.q[4 * p], x);
-                    x = T::mfmaK32(toQueryType<T>(w.y, scale), st.q[4 * p + 1], x);
-                }
+            const uint4 w = kw[tile][p];
+            x = T::mfmaK32(toQueryType<T>(w.x, k_scale[tile][p]), st.q[4 * p], x);
+            x = T::mfmaK32(toQueryType<T>(w.y, k_scale[tile][p]), st.q[4 * p + 1], x);
+            if (L::pieceWhole(p)) {
+                x = T::mfmaK32(toQueryType<T>(w.z, k_scale[tile][p]), st.q[4 * p + (L::kWords > 2 ? 2 : 0)], x);
+                x = T::mfmaK32(toQueryType<T>(w.w, k_scale[tile][p]), st.q[4 * p + (L::kWords > 2 ? 3 : 0)], x);
             }
         }
         score[tile] = x;
     }
-    auto tokenOf = [&](int j) { return 16 * (j / 4) + 4 * (j & 3) + g; }; // of the step
-    const bool masked = t0 + kStepTokens > (RUNS ? rows.least : tokens);
     const int left = (RUNS ? rows.visible : tokens) - t0; // RUNS: of row c
     if (!rows.plain) {
         const float away = static_cast<float>(1 - left);
@@ -530,75 +625,25 @@ __device__ __forceinline__ void computeStep(const Step<HEAD> &s, DecodeState<T, 
         st.l = TileF16::mfmaK32(lo, ones, st.l);
     }
 
-    // eight columns (four: COLS) of this lane, from `byte` of the rows on
-    auto columns = [&](auto cols, int byte, const float (&scale)[8], int column) {
-        constexpr int COLS = decltype(cols)::value;
-        uint32_t codes[8];
+    eachIndex<kPairs>([&](auto x) {
+        constexpr int X = decltype(x)::value;
+        uint4 even, odd;
+        operands(x, even, odd);
+        f32x4 &p0 = st.o[2 * X], &p1 = st.o[2 * X + 1];
+        p0 = TileF16::mfmaK32(hi, even, p0);
+        p1 = TileF16::mfmaK32(hi, odd, p1);
+        if constexpr (kSplit) {
+            p0 = TileF16::mfmaK32(lo, even, p0);
+            p1 = TileF16::mfmaK32(lo, odd, p1);
+        }
+        if constexpr (HEAD > 128) {
+            __builtin_amdgcn_sched_barrier(0); // one pair of operands after the other: there are no registers for all of them
+        }
+    });
+    if constexpr (RUNS) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const char *at = reinterpret_cast<const char *>(s.v) + (16 * (j / 4) + 4 * (j & 3) + g) * (HEAD / 2) + byte;
-            codes[j] = COLS == 8 ? *reinterpret_cast<const uint32_t *>(at) : *reinterpret_cast<const uint16_t *>(at);
-        }
-        auto pair = [&](auto b) {
-            constexpr int B = decltype(b)::value;
-            uint4 even, odd;
-            columnPair<B>(codes, scale, even, odd);
-            f32x4 &x = st.o[column + 2 * B], &y = st.o[column + 2 * B + 1];
-            x = TileF16::mfmaK32(hi, even, x);
-            y = TileF16::mfmaK32(hi, odd, y);
-            if constexpr (kSplit) {
-                x = TileF16::mfmaK32(lo, even, x);
-                y = TileF16::mfmaK32(lo, odd, y);
-            }
-            if constexpr (HEAD > 128) {
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        pair(std::integral_constant<int, 0>{});
-        pair(std::integral_constant<int, 1>{});
-        if constexpr (COLS == 8) {
-            pair(std::integral_constant<int, 2>{});
-            pair(std::integral_constant<int, 3>{});
-        }
-    };
-#pragma unroll
-    for (int strip = 0; strip < L::kStrips; ++strip) {
-        const int byte = L::column(strip, c) / 2; // of a row; a scale covers 16
-        float scale[8];
-#pragma unroll
-        for (int tile = 0; tile < 2; ++tile) {
-            const uint4 w = reinterpret_cast<const uint4 *>(s.vs)[(4 * tile + g) * (HEAD / 32) + byte / 16];
-            scale[4 * tile] = mx::scaleOf(w.x);
-            scale[4 * tile + 1] = mx::scaleOf(w.y);
-            scale[4 * tile + 2] = mx::scaleOf(w.z);
-            scale[4 * tile + 3] = mx::scaleOf(w.w);
-        }
-        uint32_t bad = 0; // RUNS: bit j = the value of token j is not finite
-        if (masked) {     // a NaN there would pass through a probability of zero
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const bool seen = t0 + tokenOf(j) < tokens;
-                if constexpr (RUNS) { // by some row; which ones see it is settled below
-                    const bool finite = __float_as_uint(scale[j]) != 0x7f800000u;
-                    bad |= seen && !finite ? 1u << j : 0u;
-                    scale[j] = seen && finite ? scale[j] : 0.0f;
-                } else {
-                    scale[j] = seen ? scale[j] : 0.0f;
-                }
-            }
-        }
-        if (strip == 1) {
-            columns(std::integral_constant<int, 4>{}, byte, scale, 8);
-        } else if constexpr (L::kStripCols == 4) {
-            columns(std::integral_constant<int, 4>{}, byte, scale, 0);
-        } else {
-            columns(std::integral_constant<int, 8>{}, byte, scale, 0);
-            if constexpr (L::kStripCols == 16) {
-                columns(std::integral_constant<int, 8>{}, byte + 4, scale, 8);
-            }
-        }
-        if constexpr (RUNS) {
-            if (__builtin_amdgcn_ballot_w64(bad != 0) != 0) { // the columns of this strip, in the rows that see such a token
+        for (int strip = 0; strip < L::kStrips; ++strip) {
+            if (__builtin_amdgcn_ballot_w64(bad[strip] != 0) != 0) { // the columns of this strip, in the rows that see such a token
                 int first[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -606,7 +651,7 @@ __device__ __forceinline__ void computeStep(const Step<HEAD> &s, DecodeState<T, 
                 }
 #pragma unroll
                 for (int of = 0; of < 4; ++of) {
-                    const uint32_t theirs = __shfl(bad, 16 * of + c, 64);
+                    const uint32_t theirs = __shfl(bad[strip], 16 * of + c, 64);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const int t = 16 * (j / 4) + 4 * (j & 3) + of;
@@ -735,17 +780,77 @@ __device__ __forceinline__ void finish(const DecodeState<T, HEAD> &st, const Row
     }
 }
 
+// Steps [from, to) of a segment, from nothing: what the lanes hold afterwards is theirs alone.
+template <typename T, int HEAD, int GRAIN, bool RUNS, int STAGES>
+__device__ __forceinline__ void walk(Pages<HEAD, GRAIN> &pages, Step<HEAD> (&ring)[STAGES], DecodeState<T, HEAD> &st, Rows &rows, int lane,
+                                     int kv_head, int seq, int segment, int tokens, int first_token, int q_len, int history, int from,
+                                     int to) {
+    using L = Layout<HEAD>;
+    constexpr int kStages = STAGES;
+    const int g = lane >> 4, c = lane & 15;
+    pages.begin(seq * argsAgain()->block_table_stride, tokens, from);
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) {
+        if (from + i < to) {
+            pages.load(ring[i]);
+        }
+    }
+    {
+        const ArgsAgain again = argsAgain();
+        const RowPlace place = rowPlace<RUNS>(again->group, kv_head, segment, c, first_token, q_len);
+        loadQuery<T, HEAD>(again, place, g, st.q);
+        rows.slope_log2 = !rows.plain && again->alibi_slopes != nullptr && place.exists ? again->alibi_slopes[place.head] * kLog2e : 0.0f;
+        if constexpr (RUNS) {
+            const int sees = history + (place.token - first_token) + 1;
+            rows.visible = !place.exists || sees < 0 ? 0 : (sees > tokens ? tokens : sees);
+            rows.least = __builtin_amdgcn_readfirstlane(-waveMaxInt(-(place.exists ? rows.visible : 0x7fffffff)));
+        }
+    }
+    // Used here, so that the compiler waits for the query here: left to their first use in the loop, these loads would be
+    // waited for there, by a count that knows nothing of the loads into LDS and so waits for all of those as well, in
+    // every step.
+#pragma unroll
+    for (int w = 0; w < HEAD / 32; ++w) {
+        asm volatile("" : "+v"(st.q[w].x), "+v"(st.q[w].y), "+v"(st.q[w].z), "+v"(st.q[w].w));
+    }
+    asm volatile("" : "+v"(rows.slope_log2));
+    st.m = -INFINITY;
+    st.shift = 0.0f;
+    st.l = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < HEAD / 16; ++e) {
+        st.o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    int stage = 0;
+    for (int step = from; step < to; ++step) {
+        // the loads of this step are done; those of the steps behind it, up to kStages - 1, may be under way
+        const int behind = to - 1 - step;
+        if (behind >= kStages - 1) {
+            waitLoads<(kStages - 1) * L::kLoads>();
+        } else if (kStages > 3 && behind >= 2) {
+            waitLoads<(kStages > 3 ? 2 : 0) * L::kLoads>();
+        } else if (kStages > 2 && behind >= 1) {
+            waitLoads<(kStages > 2 ? 1 : 0) * L::kLoads>();
+        } else {
+            waitLoads<0>();
+        }
+        computeStep<T, HEAD, RUNS>(ring[stage], st, rows, lane, step * kStepTokens, tokens);
+        if (step + kStages < to) {
+            pages.load(ring[stage]);
+        }
+        stage = stage + 1 < kStages ? stage + 1 : 0;
+    }
+}
+
 // Grid: KV heads x (runs / 4) x chunks of heads. Two neighbouring KV heads take turns on the dies: their scales share cache
 // lines, and a die that works on both at a time fetches them once.
 template <typename T, int HEAD, int GRAIN, bool RUNS>
 __global__ void __launch_bounds__(kDecodeThreads, Layout<HEAD>::kPerUnit)
 decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_type_, int32_t num_seqs, int32_t capacity, int32_t most_runs,
                 DecodeFp4Args a) {
-    using L = Layout<HEAD>;
-    constexpr int kStages = L::kStages;
-    __shared__ Step<HEAD> rings[kDecodeThreads / 64][kStages];
+    __shared__ Step<HEAD> rings[kDecodeThreads / 64][Layout<HEAD>::kStages];
     const IndexType index_type = static_cast<IndexType>(index_type_);
-    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     auto work = [&](int seq) { return workOf<RUNS>(index_type, seq_lens, cu_seqlens_q, capacity, RUNS ? a.total_q_tokens : 0, RUNS ? a.group : 0, seq); };
 
@@ -777,12 +882,7 @@ decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_ty
     auto &ring = rings[wave];
     Pages<HEAD, GRAIN> pages(a, lane, kv_head);
     DecodeState<T, HEAD> st;
-    Rows rows;
-    rows.plain = a.alibi_slopes == nullptr && a.scale_log2 > 0.0f;
-    rows.scale_log2 = a.scale_log2;
-    rows.unit = rows.plain ? a.scale_log2 : 1.0f;
-    rows.lazy = kLazyLog2 / rows.unit;
-    rows.visible = rows.least = 0;
+    Rows rows(a);
 
     uint32_t before = 0, segments_before = 0; // of the sequences in front of the 64 at hand
     for (int base = 0; base < num_seqs && at < end; base += 64) {
@@ -814,50 +914,7 @@ decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_ty
             const int from = static_cast<int>(at - start);
             const int to = static_cast<int>(end - start < static_cast<uint32_t>(steps) ? end - start : steps);
 
-            pages.begin(seq * argsAgain()->block_table_stride, tokens, from);
-#pragma unroll
-            for (int i = 0; i < kStages; ++i) {
-                if (from + i < to) {
-                    pages.load(ring[i]);
-                }
-            }
-            {
-                const ArgsAgain again = argsAgain();
-                const RowPlace place = rowPlace<RUNS>(again->group, kv_head, segment, c, first_token, q_len);
-                loadQuery<T, HEAD>(again, place, g, st.q);
-                rows.slope_log2 = !rows.plain && again->alibi_slopes != nullptr && place.exists ? again->alibi_slopes[place.head] * kLog2e : 0.0f;
-                if constexpr (RUNS) {
-                    const int sees = history + (place.token - first_token) + 1;
-                    rows.visible = !place.exists || sees < 0 ? 0 : (sees > tokens ? tokens : sees);
-                    rows.least = __builtin_amdgcn_readfirstlane(-waveMaxInt(-(place.exists ? rows.visible : 0x7fffffff)));
-                }
-            }
-            st.m = -INFINITY;
-            st.shift = 0.0f;
-            st.l = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int e = 0; e < HEAD / 16; ++e) {
-                st.o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
-            int stage = 0;
-            for (int step = from; step < to; ++step) {
-                // the loads of this step are done; those of the steps behind it, up to kStages - 1, may be under way
-                const int behind = to - 1 - step;
-                if (behind >= kStages - 1) {
-                    waitLoads<(kStages - 1) * L::kLoads>();
-                } else if (kStages > 3 && behind >= 2) {
-                    waitLoads<(kStages > 3 ? 2 : 0) * L::kLoads>();
-                } else if (kStages > 2 && behind >= 1) {
-                    waitLoads<(kStages > 2 ? 1 : 0) * L::kLoads>();
-                } else {
-                    waitLoads<0>();
-                }
-                computeStep<T, HEAD, RUNS>(ring[stage], st, rows, lane, step * kStepTokens, tokens);
-                if (step + kStages < to) {
-                    pages.load(ring[stage]);
-                }
-                stage = stage + 1 < kStages ? stage + 1 : 0;
-            }
+            walk<T, HEAD, GRAIN, RUNS>(pages, ring, st, rows, lane, kv_head, seq, segment, tokens, first_token, q_len, history, from, to);
             const bool whole = from == 0 && to == steps;
             if (from == 0) {
                 const ArgsAgain again = argsAgain();
@@ -871,6 +928,95 @@ decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_ty
         }
         before += all;
         segments_before += RUNS ? __builtin_amdgcn_readlane(segment_sum, 63) : 0;
+    }
+}
+
+// A whole sequence and KV head (and 16 of its query heads) by one workgroup: its eight wavefronts share the steps and join what
+// they have in LDS. Grid: KV heads x sequences x chunks of heads, neighbouring KV heads taking turns on the dies as above.
+template <typename T, int HEAD, int GRAIN>
+__global__ void __launch_bounds__(kWholeThreads, Layout<HEAD>::kWholePerUnit)
+decodeWholeFp4Kernel(const void *seq_lens, const void *, int32_t index_type, int32_t, int32_t capacity, int32_t, DecodeFp4Args a) {
+    using L = Layout<HEAD>;
+    constexpr int kWaves = kWholeThreads / 64, kLanes = HEAD / 4;
+    struct Joined { // [wave][row][column]
+        float acc[kWaves][kHeadsPerWave][HEAD];
+        float2 ml[kWaves][kHeadsPerWave];
+    };
+    __shared__ union Shared {
+        Step<HEAD> rings[kWaves][L::kWholeStages];
+        Joined joined;
+        __device__ Shared() {}
+    } shared;
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const bool paired = (gridDim.x & 1) == 0 && (gridDim.y & 1) == 0;
+    const int kv_head = paired ? (blockIdx.x & ~1u) | (blockIdx.y & 1) : blockIdx.x;
+    const int seq = paired ? (blockIdx.y & ~1u) | (blockIdx.x & 1) : blockIdx.y;
+    const int chunk = blockIdx.z;
+    const int tokens = __builtin_amdgcn_readfirstlane(workOf<false>(static_cast<IndexType>(index_type), seq_lens, nullptr, capacity, 0, 0, seq).tokens);
+    if (tokens == 0) {
+        return; // (all of the workgroup) out[seq] stays as it was
+    }
+    const Cut cut(stepsOf(tokens), kWaves);
+    Pages<HEAD, GRAIN> pages(a, lane, kv_head);
+    DecodeState<T, HEAD> st;
+    Rows rows(a);
+    const int from = cut.start(wave), to = cut.start(wave + 1);
+    st.m = -INFINITY; // of a wavefront without steps
+    if (from < to) {
+        walk<T, HEAD, GRAIN, false>(pages, shared.rings[wave], st, rows, lane, kv_head, seq, chunk, tokens, seq, 1, 0, from, to);
+    } else {
+        st.l = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < L::kCols; ++e) {
+            st.o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    __syncthreads(); // the rings are not read any more
+    const ArgsAgain again = argsAgain();
+    const int group = again->group, heads = min(group - chunk * kHeadsPerWave, kHeadsPerWave);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = 4 * g + i;
+        const float m = __shfl(st.m, r, 64);
+        if (r < heads) {
+            if (c == 0) {
+                shared.joined.ml[wave][r] = make_float2(m * rows.unit, st.l[i]);
+            }
+#pragma unroll
+            for (int e = 0; e < L::kCols; e += 4) {
+                const int strip = e < L::kStripCols ? 0 : 1;
+                *reinterpret_cast<float4 *>(&shared.joined.acc[wave][r][L::column(strip, c) + (strip == 0 ? e : e - L::kStripCols)]) =
+                    make_float4(st.o[e][i], st.o[e + 1][i], st.o[e + 2][i], st.o[e + 3][i]);
+            }
+        }
+    }
+    __syncthreads();
+    for (int at = threadIdx.x; at < heads * kLanes; at += kWholeThreads) {
+        const int r = at / kLanes, column = 4 * (at % kLanes);
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            m = maxOf(m, shared.joined.ml[w][r].x);
+        }
+        float l = 0.0f;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float2 ml = shared.joined.ml[w][r];
+            const float f = ml.x == m ? 1.0f : fastExp2(ml.x - m);
+            const float4 v = *reinterpret_cast<const float4 *>(&shared.joined.acc[w][r][column]);
+            l += ml.y * f;
+            x.x += v.x * f;
+            x.y += v.y * f;
+            x.z += v.z * f;
+            x.w += v.w * f;
+        }
+        const float f = 1.0f / l;
+        const float y[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
+        auto *row = static_cast<typename T::storage *>(again->out) + seq * again->o_stride
+                  + (kv_head * group + chunk * kHeadsPerWave + r) * again->o_head_stride;
+        storeColumns<T, 4>(row + column, y, again->out_aligned);
     }
 }
 
@@ -945,13 +1091,13 @@ __global__ void __launch_bounds__(64 * WAVES) mergeFp4Kernel(const void *seq_len
         return;
     }
     m = -INFINITY;
-#pragma unroll
+#pragma unroll 8
     for (int i = 0; i < kGroups; ++i) {
         m = maxOf(m, their_ml[i].x);
     }
     l = 0.0f;
     x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
+#pragma unroll 8
     for (int i = 0; i < kGroups; ++i) {
         const float2 ml = their_ml[i];
         const float f = ml.x == m ? 1.0f : fastExp2(ml.x - m);

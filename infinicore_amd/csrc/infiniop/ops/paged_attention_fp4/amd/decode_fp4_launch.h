@@ -12,6 +12,7 @@ namespace op::paged_attention_fp4::amd {
 // Runs of steps per stream (a KV head and up to 16 of its query heads), and where partial results lie.
 struct DecodePlan {
     bool possible;
+    bool whole;         // a workgroup per sequence and KV head: no partial results
     int head_chunks;
     int runs;           // per stream
     int part_rows;
@@ -28,6 +29,26 @@ inline int wavesPerUnit(size_t head) {
     return groups * (kDecodeThreads / 64);
 }
 
+// Whether every sequence is left to one workgroup per KV head (and 16 query heads): no scan of the lengths in front, no partial
+// results and no second kernel, but as long as the longest sequence, and whole rounds of workgroups. `steps`: of the longest
+// that the table can hold. us cut into runs / whole, bf16, lengths between half of and the given tokens:
+//   head 128, 64 / 8 heads: 500 tokens 64 workgroups 10.3 / 7.2, 256 18.3 / 7.9, 512 22.0 / 14.7, 1 024 27.7 / 27.1; 1 000 tokens 8
+//   9.1 / 8.0, 256 22.2 / 11.1, 512 26.7 / 21.3, 1 024 36.5 / 39.9; 2 000 tokens 8 10.3 / 11.0, 64 16.7 / 13.7, 256 26.4 / 16.5, 512
+//   35.3 / 30.6, 1 024 53.8 / 57.4; 4 000 tokens 64 21.1 / 22.8, 200 30.6 / 24.8, 256 35.3 / 26.0 (300 - 4 000 30.2 / 24.6), 400 43.7 /
+//   43.9 (37.2 / 38.8); 32 / 8 heads, 4 096 - 8 192 256 49.2 / 46.4, 500 - 8 192 39.1 / 42.9.
+//   head 64 (two such workgroups to a compute unit): 4 000 tokens 128 16.2 / 18.9, 192 19.8 / 20.3, 512 32.8 / 29.7; head 192: 1 000
+//   tokens 8 10.2 / 10.6, 2 000 64 18.2 / 18.6, 400 38.5 / 38.9; head 256: 1 000 tokens 8 10.8 / 11.9, 64 16.4 / 13.7.
+inline bool wholeSequences(int64_t workgroups, int64_t steps, size_t head, int compute_units) {
+    const int64_t slots = static_cast<int64_t>(compute_units) * (head == 64 ? Layout<64>::kWholePerUnit : Layout<128>::kWholePerUnit);
+    if (steps <= 32) {
+        return workgroups <= 2 * slots && (steps <= 16 || head <= 128 || 4 * workgroups >= compute_units);
+    }
+    if (steps <= 64) {
+        return workgroups <= 2 * slots && 4 * workgroups >= compute_units;
+    }
+    return steps <= 128 && workgroups <= slots && 4 * workgroups >= 3 * compute_units;
+}
+
 // `by_rows`: several query tokens per sequence (RUNS).
 inline DecodePlan planDecode(const AttentionFp4Info &in, bool by_rows, int compute_units) {
     DecodePlan plan{};
@@ -42,6 +63,11 @@ inline DecodePlan planDecode(const AttentionFp4Info &in, bool by_rows, int compu
         return plan;
     }
     plan.max_segments = static_cast<int>(segments);
+    plan.whole = !by_rows && wholeSequences(segments * streams, per_segment, in.head_size, compute_units);
+    if (plan.whole) {
+        plan.runs = 1;
+        return plan;
+    }
     const int64_t steps = segments * per_segment;
     const int64_t fill = (static_cast<int64_t>(compute_units) * wavesPerUnit(in.head_size) + streams - 1) / streams;
     plan.runs = static_cast<int>(std::max<int64_t>(1, std::min(fill, (steps + kLeastSteps - 1) / kLeastSteps)));
@@ -118,6 +144,12 @@ void launchDecode(const DecodeFp4Args &a, const DecodePlan &plan, hipStream_t st
     unsigned groups = static_cast<unsigned>((plan.runs + kWaves - 1) / kWaves);
     groups += a.num_kv_heads % 2 == 0 && groups > 1 && groups % 2 != 0 ? 1 : 0; // (pairs of KV heads: see the kernel)
 #define EARLY a.seq_lens, a.cu_seqlens_q, static_cast<int32_t>(a.index_type), a.num_seqs, a.capacity, a.runs
+    if constexpr (!RUNS) {
+        if (plan.whole) {
+            decodeWholeFp4Kernel<T, HEAD, GRAIN><<<dim3(a.num_kv_heads, a.num_seqs, plan.head_chunks), kWholeThreads, 0, stream>>>(EARLY, a);
+            return;
+        }
+    }
     decodeFp4Kernel<T, HEAD, GRAIN, RUNS><<<dim3(a.num_kv_heads, groups, plan.head_chunks), kDecodeThreads, 0, stream>>>(EARLY, a);
     if (plan.runs > 1) {
         const dim3 grid(static_cast<unsigned>(plan.max_segments) * plan.part_rows, a.num_kv_heads, plan.head_chunks);

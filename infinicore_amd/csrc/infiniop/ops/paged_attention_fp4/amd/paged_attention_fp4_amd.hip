@@ -80,7 +80,8 @@ infiniStatus_t Descriptor::calculate(void *workspace, size_t workspace_size, voi
     }
     auto address = [](const void *p) { return reinterpret_cast<uintptr_t>(p); };
     const size_t index_bytes = infiniSizeOf(in.index_dtype);
-    if ((address(k_codes) | address(v_codes)) % 16 != 0 || (address(q) | address(out)) % 2 != 0
+    if ((address(k_codes) | address(v_codes)) % 16 != 0 || (address(k_scales) | address(v_scales)) % in.scaleBytes() != 0
+        || (address(q) | address(out)) % 2 != 0
         || (address(block_tables) | address(seq_lens)) % index_bytes != 0 || address(alibi_slopes) % 4 != 0) {
         return INFINI_STATUS_BAD_PARAM;
     }

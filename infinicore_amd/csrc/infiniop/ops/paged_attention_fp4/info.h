@@ -98,8 +98,9 @@ struct AttentionFp4Info {
             || (alibi_slopes_desc != nullptr && alibi_slopes_desc->dim(0) < info.num_heads)) {
             return INFINI_STATUS_BAD_TENSOR_SHAPE;
         }
-        // the kernels load 16 bytes of codes at a time, and their offsets inside a page are of 32 bits
+        // the kernels load 16 bytes of codes and up to four scales at a time, and their offsets inside a page are of 32 bits
         CHECK_OR_RETURN(info.pool.codeRowsAligned(16), INFINI_STATUS_BAD_TENSOR_STRIDES);
+        CHECK_OR_RETURN(info.pool.scaleRowsAligned(info.scaleBytes()), INFINI_STATUS_BAD_TENSOR_STRIDES);
         const fp4::PoolInfo &p = info.pool;
         for (ptrdiff_t row : {p.k_codes.row, p.v_codes.row, p.k_scales.row, p.v_scales.row}) {
             CHECK_OR_RETURN(row >= 0 && row <= 0xffffff, INFINI_STATUS_BAD_TENSOR_STRIDES);
@@ -119,6 +120,9 @@ struct AttentionFp4Info {
         info.block_table_batch_stride = block_tables_desc->stride(0);
         return info;
     }
+
+    // Scales that are loaded at a time: a row's, where it has two or four, else a part of them.
+    size_t scaleBytes() const { return head_size % 128 == 0 ? 4 : 2; }
 
     // Tokens that a row of the block table can hold, at most 2^30.
     int capacity() const {
