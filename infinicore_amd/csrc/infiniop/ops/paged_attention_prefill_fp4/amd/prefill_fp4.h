@@ -2,16 +2,18 @@
 // 256.
 //
 // One 256-thread workgroup = 64 R "rows" of one (sequence, KV head); a row is a (new token, query head of the group) pair,
-// token-major. Each wavefront owns 16 R rows. The tokens that the rows may see are consumed in steps of 64 (32 at head 192
-// with R = 1): per step each wavefront loads the codes and scales of its share of the tokens, a step ahead, into registers,
-// turns them into 16-bit values between the matrix instructions of the present step (v_cvt_scalef32_pk_*, two elements per
-// instruction; K in the query's type, V in fp16, where every written value is exact) and leaves them in LDS for everybody;
-// one barrier per step. lane = 16 g + c:
-//   S[token][row] = K . Q^T   v_mfma_f32_16x16x32 (A = K out of LDS, B = Q in registers; lane holds S[16 T + 4g + 0..3][row c])
+// token-major. Each wavefront owns 16 R rows. The tokens that the rows may see are consumed in steps of 64: per step each
+// wavefront loads the codes and scales of 16 of them, two steps ahead, into registers, and a step ahead leaves them in LDS for
+// everybody, between the matrix instructions: K as it is, V as fp16, where every written value is exact
+// (v_cvt_scalef32_pk_*, two elements per instruction); one barrier per step. lane = 16 g + c:
+//   S[token][row] = K . Q^T   v_mfma_scale_f32_16x16x128 (A = codes and scales of K out of LDS, B = Q in three 6-bit terms in
+//                             registers: see Terms; lane holds S[16 T + 4g + 0..3][row c])
 //   causal mask (only in steps that touch the diagonal), online softmax in fp32 / log2 domain
 //   O[dim][row] += V . P      v_mfma_f32_16x16x32 (A = V by the transposing LDS read; B = P in fp16 as S came out;
 //                             lane holds O[16 e + 4g + 0..3][row c])
 //   l[row]      += 1 . P      v_mfma_f32_16x16x32
+// K in 16 bits (converted like V, four 16-bit products to the three) took 507 us where this takes 459: 16 sequences, 128 - 512
+// new tokens over 1 024 - 8 192 cached, 32 / 8 heads of 128; its LDS traffic is 4 / 5 of the other's 160 KB a step.
 // A value that is not finite has scale 255: it goes into LDS as zero, its token is noted, and the outputs of the rows that
 // see that token become NaN in the columns of its group; rows that do not see it are not touched by it.
 #ifndef INFINICORE_AMD_PA_PREFILL_FP4_H
@@ -35,7 +37,6 @@ using op::paged_attention_fp4::amd::IndexType;
 using op::paged_attention_fp4::amd::loadIndexOf;
 using op::paged_attention_fp4::amd::loadWords;
 using op::paged_attention_fp4::amd::PoolSide;
-using op::paged_attention_fp4::amd::toQueryType;
 namespace mx = device::amd::mx;
 
 constexpr int kPrefillThreads = 256;
@@ -116,42 +117,48 @@ __device__ __forceinline__ bool findBlock(const PrefillFp4Args &a, int lane, int
     return false;
 }
 
-// A head's rows in LDS and in the lanes that fill it. A unit is what a lane converts: 32 elements (16 at head 64, so that
-// the 64 lanes have a tile's 16 tokens between them) under one scale.
+// A head's rows in LDS and in the lanes that fill it. K: a lane has 16 bytes of codes, 32 elements under one scale. V: a unit is
+// what a lane converts, 32 elements (16 at head 64, so that the 64 lanes have a tile's 16 tokens between them) under one scale.
 template <int HEAD>
 struct Rows {
+    using K = op::paged_attention_fp4::amd::Layout<HEAD>; // codes of K lie in LDS as those of decode do
+    static constexpr int kGroups = HEAD / 32;          // scales of a row, and chunks of its codes
+    static constexpr int kPassesK = (kGroups + 3) / 4; // of 64 lanes over a tile
     static constexpr int kUnit = HEAD == 64 ? 16 : 32;
     static constexpr int kUnitWords = kUnit / 8;       // dwords of codes
     static constexpr int kUnits = HEAD / kUnit;        // of a token: 4, 4, 6, 8
     static constexpr int kPasses = (kUnits + 3) / 4;   // of 64 lanes over a tile
-    static constexpr int kChunks = HEAD / 8;           // 16-byte chunks of a row
+    static constexpr int kChunks = HEAD / 8;           // 16-byte chunks of a row of 16-bit values
     static constexpr int kSwizzle = HEAD % 128 == 0 ? 16 : 8;
     static constexpr int kCols = HEAD / 16;            // blocks of 16 columns
-    static constexpr int kGroups = HEAD / 32;          // scales of a row
-    // K: row-major, chunks swizzled by the row
-    static __device__ __forceinline__ int kSlot(int row, int chunk) { return row * kChunks + (chunk ^ (row & (kSwizzle - 1))); }
     // V: [row half (8 rows)][block of 16 columns][row of the half][two chunks, exchanged in the upper half], so that neither
     // the transposing reads nor the writes of 16 tokens meet in a bank
     static __device__ __forceinline__ int vSlot(int row, int chunk) {
         return (row >> 3) * 8 * kChunks + (chunk >> 1) * 16 + (row & 7) * 2 + ((chunk & 1) ^ (row >> 3));
     }
+    // K . Q^T: the three terms of Q are laid end to end, 3 kGroups groups of 32 elements, four to an instruction (its lanes
+    // 16 g .. 16 g + 15 have group 4 m + g); the chunks of K go round beneath them, and after kSets instructions as before.
+    static constexpr int kProducts = (3 * kGroups + 3) / 4;               // instructions: 2, 3, 5, 6
+    static constexpr int kSets = kGroups < 4 ? 1 : (kGroups % 4 == 0 ? kGroups / 4 : kGroups / 2); // 1, 1, 3, 2
+    static __device__ __forceinline__ int chunkOf(int set, int g) { return (4 * set + g) % kGroups; }
+    static __device__ __forceinline__ int termOf(int m, int g) { return (4 * m + g) / kGroups; } // 3: none
 };
 
-// Tokens per step: 64, but 32 at head 192 with 64 rows, where two workgroups then share a compute unit's LDS.
-template <int HEAD, int R>
-constexpr int stepTokens() { return HEAD == 192 && R == 1 ? 32 : 64; }
-template <int HEAD, int R>
-constexpr int workgroupsPerUnit() { return HEAD <= 128 || (HEAD == 192 && R == 1) ? 2 : 1; }
+constexpr int kStep = 64, kTiles = kStep / kTile; // tokens per step
+template <int HEAD>
+constexpr int kPerUnit = HEAD < 256 ? 2 : 1; // workgroups that share a compute unit (its LDS, at head 256)
 
 // WHOLE: the page size is a multiple of 16, so that a tile lies in one page; otherwise every lane looks its rows up.
 template <typename T, int HEAD, int R, bool WHOLE>
-__global__ void __launch_bounds__(kPrefillThreads, (workgroupsPerUnit<HEAD, R>())) prefillFp4Kernel(PrefillFp4Args a) {
+__global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Kernel(PrefillFp4Args a) {
     using S = typename T::storage;
     using G = Rows<HEAD>;
-    constexpr int BM = 64 * R, BN = stepTokens<HEAD, R>(), TT = BN / kTile;
+    constexpr int BM = 64 * R, BN = kStep, TT = kTiles;
     constexpr int kTileSlots = kTile * G::kChunks;
     struct Tiles {
-        uint4 k[2][TT * kTileSlots], v[2][TT * kTileSlots];
+        uint4 k[2][BN * G::kGroups];         // codes
+        uint32_t k_scales[2][kTile * G::kGroups]; // [group][token of a tile]: byte i = tile i
+        uint4 v[2][TT * kTileSlots];         // fp16
     };
     __shared__ Tiles tiles;
     // values that are not finite: bit t of [step % 3][scale group] = token t of the step
@@ -184,7 +191,8 @@ __global__ void __launch_bounds__(kPrefillThreads, (workgroupsPerUnit<HEAD, R>()
     }
 
     // ---- this lane's columns: row c of each of the wavefront's R groups of 16 rows ----
-    uint4 q_reg[R][HEAD / 32];
+    mx::u32x6 q_codes[R][G::kProducts];
+    uint32_t q_scales[R][(G::kProducts + 3) / 4]; // bytes
     int visible[R];
     float slope[R];
     int most_visible = 0, least_visible = 0x7fffffff;
@@ -198,16 +206,45 @@ __global__ void __launch_bounds__(kPrefillThreads, (workgroupsPerUnit<HEAD, R>()
         slope[r] = a.alibi_slopes != nullptr && valid ? a.alibi_slopes[head] * kLog2e : 0.0f;
         const S *from = static_cast<const S *>(a.q) + (span.q_start + token) * a.q_stride + head * a.q_head_stride;
 #pragma unroll
-        for (int kk = 0; kk < HEAD / 32; ++kk) {
-            const S *at = from + 32 * kk + 8 * g;
-            uint4 x;
-            if (a.q_aligned) {
-                x = *reinterpret_cast<const uint4 *>(at);
-            } else {
-                const uint16_t *e = reinterpret_cast<const uint16_t *>(at);
-                x = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        for (int i = 0; i < (G::kProducts + 3) / 4; ++i) {
+            q_scales[r][i] = 0;
+        }
+#pragma unroll
+        for (int set = 0; set < G::kSets; ++set) {
+            const S *at = from + 32 * G::chunkOf(set, g);
+            mx::f32x16 even, odd;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t x[4];
+                if (a.q_aligned) {
+                    const uint4 y = reinterpret_cast<const uint4 *>(at)[i];
+                    x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
+                } else {
+                    const uint16_t *e = reinterpret_cast<const uint16_t *>(at) + 8 * i;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        x[j] = e[2 * j] | static_cast<uint32_t>(e[2 * j + 1]) << 16;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t pair = valid ? x[j] : 0u;
+                    even[4 * i + j] = T::toFloat(__builtin_bit_cast(S, static_cast<uint16_t>(pair)));
+                    odd[4 * i + j] = T::toFloat(__builtin_bit_cast(S, static_cast<uint16_t>(pair >> 16)));
+                }
             }
-            q_reg[r][kk] = valid ? x : make_uint4(0, 0, 0, 0);
+            const mx::Terms terms = mx::termsOf(even, odd);
+#pragma unroll
+            for (int m = set; m < G::kProducts; m += G::kSets) {
+                const int term = G::termOf(m, g);
+                mx::u32x6 codes;
+#pragma unroll
+                for (int i = 0; i < 6; ++i) {
+                    codes[i] = term == 0 ? terms.codes[0][i] : term == 1 ? terms.codes[1][i] : term == 2 ? terms.codes[2][i] : 0u;
+                }
+                q_codes[r][m] = codes;
+                q_scales[r][m / 4] |= (term == 0 ? terms.scale[0] : term == 1 ? terms.scale[1] : terms.scale[2]) << (8 * (m % 4));
+            }
         }
         most_visible = max(most_visible, visible[r]);
         least_visible = min(least_visible, valid ? visible[r] : 0x7fffffff);
@@ -215,25 +252,25 @@ __global__ void __launch_bounds__(kPrefillThreads, (workgroupsPerUnit<HEAD, R>()
     most_visible = __builtin_amdgcn_readfirstlane(waveMaxInt(most_visible));
     least_visible = __builtin_amdgcn_readfirstlane(-waveMaxInt(-least_visible));
 
-    // ---- loads: codes and scales of this wavefront's tile of a step (TT = 4: tile w of K and V; TT = 2: wavefronts 0, 1 take
-    // the tiles of K, 2, 3 those of V) ----
-    const bool loads_k = TT == 4 || w < 2, loads_v = TT == 4 || w >= 2;
-    const int own_tile = TT == 4 ? w : (w & 1);
+    // ---- loads: codes and scales of this wavefront's tile of a step ----
+    const int own_tile = w;
     const int64_t table_row = seq * a.block_table_stride;
     const int last_entry = (block_visible - 1) / a.block_size;
     auto entryId = [&](int entry) { return clampPage(loadIndexOf(a.index_type, a.block_tables, table_row + min(entry, last_entry)), a.num_blocks); };
 
     struct Raw { // what a lane has loaded, per pass
-        uint32_t k[G::kPasses][G::kUnitWords], v[G::kPasses][G::kUnitWords];
-        uint32_t ks[G::kPasses], vs[G::kPasses];
+        uint32_t k[G::kPassesK][4], v[G::kPasses][G::kUnitWords];
+        uint32_t ks[G::kPassesK], vs[G::kPasses];
     };
     Raw raw;
-    // which row of the tile and which unit of it this lane has: K unit-fastest (contiguous loads), V token-fastest (see vSlot)
-    auto kRow = [&](int p) { return (64 * p + lane) / G::kUnits; };
-    auto kUnitOf = [&](int p) { return (64 * p + lane) % G::kUnits; };
+    // which row of the tile and which chunk or unit of it this lane has: K chunk-fastest (contiguous loads), V token-fastest
+    // (see vSlot)
+    auto kRow = [&](int p) { return (64 * p + lane) / G::kGroups; };
+    auto kChunkOf = [&](int p) { return (64 * p + lane) % G::kGroups; };
+    auto hasK = [&](int p) { return 64 * p + lane < kTile * G::kGroups; };
     auto vRow = [&](int p) { return lane & 15; };
     auto vUnitOf = [&](int p) { return (64 * p + lane) >> 4; };
-    auto has = [&](int p) { return 64 * p + lane < kTile * G::kUnits; };
+    auto hasV = [&](int p) { return 64 * p + lane < kTile * G::kUnits; };
 
     // table entries of 64 pages, a batch ahead (WHOLE)
     int batch = 0, ids = 0, ids_next = 0;
@@ -263,79 +300,71 @@ __global__ void __launch_bounds__(kPrefillThreads, (workgroupsPerUnit<HEAD, R>()
             }
             const int64_t id = __builtin_amdgcn_readlane(ids, e & 63);
             auto tile = [&](const PoolSide &s) { return s.base + id * s.block + kv_head * s.head + static_cast<int64_t>(row0) * s.row; };
-            if (loads_k) {
-                const char *codes = tile(a.k_codes), *scales = tile(a.k_scales);
+            const char *k_codes = tile(a.k_codes), *k_scales = tile(a.k_scales);
 #pragma unroll
-                for (int p = 0; p < G::kPasses; ++p) {
-                    if (has(p)) {
-                        loadWords<4 * G::kUnitWords, false>(codes + kRow(p) * a.k_codes.row + kUnitOf(p) * (G::kUnit / 2), raw.k[p]);
-                        raw.ks[p] = static_cast<uint8_t>(scales[kRow(p) * a.k_scales.row + kUnitOf(p) * G::kUnit / 32]);
-                    }
+            for (int p = 0; p < G::kPassesK; ++p) {
+                if (hasK(p)) {
+                    loadWords<16, false>(k_codes + kRow(p) * a.k_codes.row + 16 * kChunkOf(p), raw.k[p]);
+                    raw.ks[p] = static_cast<uint8_t>(k_scales[kRow(p) * a.k_scales.row + kChunkOf(p)]);
                 }
             }
-            if (loads_v) {
-                const char *codes = tile(a.v_codes), *scales = tile(a.v_scales);
+            const char *v_codes = tile(a.v_codes), *v_scales = tile(a.v_scales);
 #pragma unroll
-                for (int p = 0; p < G::kPasses; ++p) {
-                    if (has(p)) {
-                        loadWords<4 * G::kUnitWords, false>(codes + vRow(p) * a.v_codes.row + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
-                        raw.vs[p] = static_cast<uint8_t>(scales[vRow(p) * a.v_scales.row + vUnitOf(p) * G::kUnit / 32]);
-                    }
+            for (int p = 0; p < G::kPasses; ++p) {
+                if (hasV(p)) {
+                    loadWords<4 * G::kUnitWords, false>(v_codes + vRow(p) * a.v_codes.row + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
+                    raw.vs[p] = static_cast<uint8_t>(v_scales[vRow(p) * a.v_scales.row + vUnitOf(p) * G::kUnit / 32]);
                 }
             }
         } else {
             auto rowOf = [&](const PoolSide &s, int64_t id, int row) { return s.base + id * s.block + kv_head * s.head + static_cast<int64_t>(row) * s.row; };
 #pragma unroll
+            for (int p = 0; p < G::kPassesK; ++p) {
+                if (hasK(p)) {
+                    const int token = min(t + kRow(p), block_visible - 1), e = token / a.block_size;
+                    const int id = entryId(e), row = token - e * a.block_size;
+                    loadWords<16, false>(rowOf(a.k_codes, id, row) + 16 * kChunkOf(p), raw.k[p]);
+                    raw.ks[p] = static_cast<uint8_t>(rowOf(a.k_scales, id, row)[kChunkOf(p)]);
+                }
+            }
+#pragma unroll
             for (int p = 0; p < G::kPasses; ++p) {
-                if (has(p)) {
-                    if (loads_k) {
-                        const int token = min(t + kRow(p), block_visible - 1), e = token / a.block_size;
-                        const int id = entryId(e), row = token - e * a.block_size;
-                        loadWords<4 * G::kUnitWords, false>(rowOf(a.k_codes, id, row) + kUnitOf(p) * (G::kUnit / 2), raw.k[p]);
-                        raw.ks[p] = static_cast<uint8_t>(rowOf(a.k_scales, id, row)[kUnitOf(p) * G::kUnit / 32]);
-                    }
-                    if (loads_v) {
-                        const int token = min(t + vRow(p), block_visible - 1), e = token / a.block_size;
-                        const int id = entryId(e), row = token - e * a.block_size;
-                        loadWords<4 * G::kUnitWords, false>(rowOf(a.v_codes, id, row) + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
-                        raw.vs[p] = static_cast<uint8_t>(rowOf(a.v_scales, id, row)[vUnitOf(p) * G::kUnit / 32]);
-                    }
+                if (hasV(p)) {
+                    const int token = min(t + vRow(p), block_visible - 1), e = token / a.block_size;
+                    const int id = entryId(e), row = token - e * a.block_size;
+                    loadWords<4 * G::kUnitWords, false>(rowOf(a.v_codes, id, row) + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
+                    raw.vs[p] = static_cast<uint8_t>(rowOf(a.v_scales, id, row)[vUnitOf(p) * G::kUnit / 32]);
                 }
             }
         }
     };
-    // What was loaded for `step`, as 16-bit values in LDS. Rows that nobody of the block sees (behind the sequence's end, or
-    // behind the block's last row) may hold anything: their scores are masked, their values go in as zeros.
+    // What was loaded for `step`, in LDS: K as it is, V as 16-bit values. Rows that nobody of the block sees (behind the
+    // sequence's end, or behind the block's last row) may hold anything: their scores are masked, their values go in as zeros.
     auto convert = [&](int step) {
-        if (loads_k) {
-            uint4 *to = tiles.k[step & 1] + own_tile * kTileSlots;
+        uint4 *k_to = tiles.k[step & 1] + own_tile * (kTile * G::kGroups);
+        uint8_t *scales_to = reinterpret_cast<uint8_t *>(tiles.k_scales[step & 1]) + own_tile;
 #pragma unroll
-            for (int p = 0; p < G::kPasses; ++p) {
-                if (has(p)) {
-#pragma unroll
-                    for (int i = 0; i < G::kUnitWords; ++i) {
-                        to[G::kSlot(kRow(p), G::kUnitWords * kUnitOf(p) + i)] = toQueryType<T>(raw.k[p][i], mx::scaleOf(raw.ks[p]));
-                    }
-                }
+        for (int p = 0; p < G::kPassesK; ++p) {
+            if (hasK(p)) {
+                k_to[G::K::kSlot(kRow(p), kChunkOf(p))] = make_uint4(raw.k[p][0], raw.k[p][1], raw.k[p][2], raw.k[p][3]);
+                scales_to[4 * (kTile * kChunkOf(p) + kRow(p))] = static_cast<uint8_t>(raw.ks[p]);
             }
         }
-        if (loads_v) {
-            uint4 *to = tiles.v[step & 1] + own_tile * kTileSlots;
-            const int t = kTile * own_tile;
+        uint4 *to = tiles.v[step & 1] + own_tile * kTileSlots;
+        const int t = kTile * own_tile;
 #pragma unroll
-            for (int p = 0; p < G::kPasses; ++p) {
-                if (has(p)) {
-                    const bool seen = step * BN + t + vRow(p) < block_visible;
-                    const bool finite = raw.vs[p] != 0xff;
-                    const float scale = seen && finite ? mx::scaleOf(raw.vs[p]) : 0.0f;
+        for (int p = 0; p < G::kPasses; ++p) {
+            if (hasV(p)) {
+                const bool seen = step * BN + t + vRow(p) < block_visible;
+                const bool finite = raw.vs[p] != 0xff;
+                const float scale = seen && finite ? mx::scaleOf(raw.vs[p]) : 0.0f;
 #pragma unroll
-                    for (int i = 0; i < G::kUnitWords; ++i) {
-                        to[G::vSlot(vRow(p), G::kUnitWords * vUnitOf(p) + i)] = mx::toF16x8(raw.v[p][i], scale);
-                    }
-                    if (seen && !finite) {
-                        atomicOr(&bad[step % 3][vUnitOf(p) * G::kUnit / 32], 1ull << (t + vRow(p)));
-                        any_bad[step % 3] = 1;
-                    }
+                for (int i = 0; i < G::kUnitWords; ++i) {
+                    to[G::vSlot(vRow(p), G::kUnitWords * vUnitOf(p) + i)] = mx::toF16x8(raw.v[p][i], scale);
+                }
+                if (seen && !finite) {
+                    atomicOr(&bad[step % 3][vUnitOf(p) * G::kUnit / 32], 1ull << (t + vRow(p)));
+                    any_bad[step % 3] = 1;
                 }
             }
         }
@@ -369,18 +398,27 @@ __global__ void __launch_bounds__(kPrefillThreads, (workgroupsPerUnit<HEAD, R>()
     auto compute = [&](int step, auto between) {
         const int buf = step & 1, t0 = step * BN;
         f32x4 s[R][TT];
+        uint32_t k_scales[G::kSets];
+#pragma unroll
+        for (int set = 0; set < G::kSets; ++set) {
+            k_scales[set] = tiles.k_scales[buf][kTile * G::chunkOf(set, g) + c];
+        }
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
+            uint4 k[G::kSets];
+#pragma unroll
+            for (int set = 0; set < G::kSets; ++set) {
+                k[set] = tiles.k[buf][tt * (kTile * G::kGroups) + G::K::kSlot(c, G::chunkOf(set, g))];
+            }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 s[r][tt] = f32x4{0.f, 0.f, 0.f, 0.f};
             }
 #pragma unroll
-            for (int kk = 0; kk < HEAD / 32; ++kk) {
-                const uint4 k = tiles.k[buf][tt * kTileSlots + G::kSlot(c, 4 * kk + g)];
+            for (int m = 0; m < G::kProducts; ++m) {
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
-                    s[r][tt] = T::mfmaK32(k, q_reg[r][kk], s[r][tt]);
+                    s[r][tt] = mx::mfmaScaled(k[m % G::kSets], k_scales[m % G::kSets], tt, q_codes[r][m], q_scales[r][m / 4], m % 4, s[r][tt]);
                 }
             }
         }
