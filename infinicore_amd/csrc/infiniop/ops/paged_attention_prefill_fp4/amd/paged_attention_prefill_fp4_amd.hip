@@ -21,26 +21,27 @@ using op::paged_attention_fp4::amd::planDecode;
 using op::paged_attention_fp4::amd::rowsAligned;
 using op::paged_attention_fp4::amd::sideOf;
 
-template <typename T, int HEAD, int R>
+// Workgroups of a call, at most: every sequence has at most one row block that is not full.
+int64_t workgroups(int64_t rows, int64_t seqs, int64_t kv_heads, int block_rows) { return (rows / block_rows + seqs) * kv_heads; }
+
+template <typename T, int HEAD, int R, int WAVES>
 void launchRows(const PrefillFp4Args &a, hipStream_t stream) {
-    constexpr int BM = 64 * R;
-    // every sequence has at most one row block that is not full
-    const int64_t blocks = static_cast<int64_t>(a.total_q_tokens) * a.group / BM + a.num_seqs;
-    const dim3 grid(static_cast<unsigned>(blocks * a.num_kv_heads));
+    const int64_t rows = static_cast<int64_t>(a.total_q_tokens) * a.group;
+    const dim3 grid(static_cast<unsigned>(workgroups(rows, a.num_seqs, a.num_kv_heads, 16 * R * WAVES)));
     if (a.block_size % kTile == 0) {
-        prefillFp4Kernel<T, HEAD, R, true><<<grid, kPrefillThreads, 0, stream>>>(a);
+        prefillFp4Kernel<T, HEAD, R, WAVES, true><<<grid, 64 * WAVES, 0, stream>>>(a);
     } else {
-        prefillFp4Kernel<T, HEAD, R, false><<<grid, kPrefillThreads, 0, stream>>>(a);
+        prefillFp4Kernel<T, HEAD, R, WAVES, false><<<grid, 64 * WAVES, 0, stream>>>(a);
     }
 }
 
 template <typename T>
 void launchType(const PrefillFp4Args &a, size_t head, bool wide, hipStream_t stream) {
     switch (head) {
-    case 64: wide ? launchRows<T, 64, 2>(a, stream) : launchRows<T, 64, 1>(a, stream); break;
-    case 128: wide ? launchRows<T, 128, 2>(a, stream) : launchRows<T, 128, 1>(a, stream); break;
-    case 192: launchRows<T, 192, 1>(a, stream); break;
-    default: launchRows<T, 256, 1>(a, stream); break;
+    case 64: wide ? launchRows<T, 64, 2, 4>(a, stream) : launchRows<T, 64, 1, 4>(a, stream); break;
+    case 128: wide ? launchRows<T, 128, 2, 4>(a, stream) : launchRows<T, 128, 1, 4>(a, stream); break;
+    case 192: launchRows<T, 192, 1, 4>(a, stream); break;
+    default: wide ? launchRows<T, 256, 1, 8>(a, stream) : launchRows<T, 256, 1, 4>(a, stream); break;
     }
 }
 
@@ -64,17 +65,36 @@ void launchFewType(const DecodeFp4Args &a, size_t head, const DecodePlan &plan, 
     }
 }
 
+// Row blocks of 128 instead of 64 (heads of 64 and 128: two groups of 16 rows a wavefront, head 256: eight wavefronts), where
+// they are many enough. Heads of 64 and 128, from two workgroups of 128 rows for each compute unit on, us 64 / 128 rows, head 128,
+// 32 / 8 heads: 16 sequences over 4 000 tokens with 64 new ones each (1 workgroup a unit) 88.0 / 87.0, 96 117 / 122, 128 (2) 160 /
+// 130, 160 188 / 190; 2 prompts of 2 000 86.0 / 81.6, 3 of them 123 / 111; 1 x 512 over 8 000 (1/2) 118 / 158. Head 256, whose LDS
+// holds one workgroup, where those of 64 rows are more than the units: 2 sequences of 256 over 4 000 (1) 102 / 121, 3 (1.5) 194 /
+// 129, 8 392 / 260, 2 prompts of 2 000 243 / 155. (Head 192 took the same in both: 64 rows.)
+bool wideBlocks(const PagedAttentionPrefillFp4Info &in, int units) {
+    const int64_t rows = static_cast<int64_t>(in.num_rows * in.num_heads); // of all KV heads
+    return in.head_size == 256 ? rows / 64 > units : rows / 128 >= 2 * units;
+}
+
+// The longest row blocks first where they take more than one round: us in the order of the sequences / by length, head 128, 32 / 8
+// heads: 8 sequences of 128 - 384 over 1 000 - 8 000 tokens 246 / 202, 16 378 / 343, 40 1 055 / 1 009, 4 prompts of 1 100 - 2 400
+// 128 / 124; alike ones (64 over 0 - 4 000, 16 prompts of 2 000) 694 / 695, 576 / 579; less than a round 38.8 / 39.9.
+bool byLength(const PagedAttentionPrefillFp4Info &in, int units) {
+    return in.num_seqs <= 64 && static_cast<int64_t>(in.num_rows * in.num_heads) / 64 > units;
+}
+
 // Whether rows of 16, whose tokens the wavefronts of the whole chip divide among themselves (decode_fp4.h), beat row blocks
-// of 64 that each walk all of theirs. A row block takes 1.2 us per 64 tokens on its own and 0.66 us of a compute unit's time;
+// of 64 that each walk all of theirs. A row block takes 0.9 us per 64 tokens on its own and 0.6 us of a compute unit's time;
 // 16 rows take 0.36 us of it, and dividing and joining 12 us. (Head 128; how much a table holds stands for the lengths.)
-// Measured, row blocks / rows of 16, in us: 32 sequences of 6000 tokens, 8 KV heads: 8 rows each 121 / 54, 32 rows 121 / 91,
-// 64 rows 121 / 141; of 1000 tokens: 8 rows 26 / 22, 32 rows 27 / 32; 1 sequence of 20000: 128 rows 380 / 46.
+// Measured, row blocks / rows of 16, in us: 32 sequences of 6000 tokens, 8 KV heads: 8 rows each 89 / 55, 32 rows 90 / 86 - 97,
+// 64 rows 92 / 145; of 1000 tokens: 8 rows 23 / 22, 32 rows 24 / 33; 1 sequence of 20000: 128 rows 270 / 45; head 64: 32 of 6000, 8
+// rows 80 / 42, 64 rows 82 / 109; head 256: 142 / 94, 147 / 235.
 bool fewRows(const PagedAttentionPrefillFp4Info &in, int units) {
-    const double steps = std::max(1.0, static_cast<double>(in.capacity()) / 64);
+    const double steps = (0.6 + 0.4 / 128 * static_cast<double>(in.head_size)) * std::max(1.0, static_cast<double>(in.capacity()) / 64);
     const double seqs = static_cast<double>(in.num_seqs), rows = static_cast<double>(in.num_rows * in.num_heads / in.pool.num_kv_heads);
     const double heads_per_unit = static_cast<double>(in.pool.num_kv_heads) / units;
     const double blocks = seqs * std::ceil(rows / seqs / 64) * heads_per_unit, chunks = seqs * std::ceil(rows / seqs / 16) * heads_per_unit;
-    return 12 + 0.36 * steps * chunks < steps * std::max(1.2, 0.66 * blocks);
+    return 12 + 0.36 * steps * chunks < steps * std::max(0.9, 0.6 * blocks);
 }
 
 } // namespace
@@ -83,6 +103,7 @@ struct Descriptor::Opaque {
     bool few;        // the decode kernels, by `plan`
     DecodePlan plan;
     bool wide;       // 128 rows per workgroup
+    bool by_length;  // the longest row blocks first
 };
 
 Descriptor::~Descriptor() { delete _opaque; }
@@ -100,11 +121,11 @@ infiniStatus_t Descriptor::create(infiniopHandle_t handle, Descriptor **desc_ptr
     const PagedAttentionPrefillFp4Info in = info.take();
     const int units = device::amd::deviceInfo(handle->device_id).compute_units;
     Opaque o{};
-    const int64_t rows = static_cast<int64_t>(in.num_rows * in.num_heads); // of all KV heads
-    o.wide = rows / 128 >= 2 * units;
+    o.wide = wideBlocks(in, units);
+    o.by_length = byLength(in, units);
     if (fewRows(in, units)) {
         o.plan = planDecode(in, true, units);
-        o.few = o.plan.possible && static_cast<int64_t>(o.plan.max_segments) * o.plan.part_rows <= 0x7fffffff; // (the merge's grid)
+        o.few = o.plan.possible && static_cast<int64_t>(o.plan.max_segments) * o.plan.part_rows < 0x400000; // (2^32 threads of the merge)
     }
     *desc_ptr = new Descriptor(new Opaque{o}, in, o.few ? o.plan.workspaceBytes() : 0, handle->device, handle->device_id);
     return INFINI_STATUS_SUCCESS;
@@ -175,6 +196,7 @@ infiniStatus_t Descriptor::calculate(void *workspace, size_t workspace_size, voi
     a.block_size = static_cast<int32_t>(in.pool.block_size);
     a.num_blocks = static_cast<int32_t>(std::min<size_t>(in.pool.num_blocks, 0x7fffffff));
     a.capacity = in.capacity();
+    a.by_length = _opaque->by_length;
     a.q_aligned = rowsAligned(q, in.q_stride, in.q_head_stride);
     a.out_aligned = rowsAligned(out, in.o_stride, in.o_head_stride);
     a.q_stride = in.q_stride;

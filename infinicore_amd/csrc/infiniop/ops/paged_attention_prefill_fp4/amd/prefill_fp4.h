@@ -1,7 +1,7 @@
 // Prefill kernel over a KV pool held in 4 bits, gfx950 (CDNA4, 64-lane wavefronts), head_size = value_size = 64, 128, 192 or
 // 256.
 //
-// One 256-thread workgroup = 64 R "rows" of one (sequence, KV head); a row is a (new token, query head of the group) pair,
+// One workgroup of four or eight wavefronts = 64 R or 128 R "rows" of one (sequence, KV head); a row is a (new token, query head of the group) pair,
 // token-major. Each wavefront owns 16 R rows. The tokens that the rows may see are consumed in steps of 64: per step each
 // wavefront loads the codes and scales of 16 of them, two steps ahead, into registers, and a step ahead leaves them in LDS for
 // everybody, between the matrix instructions: K as it is, V as fp16, where every written value is exact
@@ -39,7 +39,6 @@ using op::paged_attention_fp4::amd::loadWords;
 using op::paged_attention_fp4::amd::PoolSide;
 namespace mx = device::amd::mx;
 
-constexpr int kPrefillThreads = 256;
 constexpr int kTile = 16;          // tokens of a matrix instruction
 constexpr float kLazyLog2 = 8.0f;  // how far (in powers of two) a row maximum may outgrow its reference point
 
@@ -58,6 +57,7 @@ struct PrefillFp4Args {
     int32_t block_size;
     int32_t num_blocks; // pool size; table entries are clamped into [0, num_blocks)
     int32_t capacity;   // tokens that a row of the block table can hold, at most
+    bool by_length;     // the longest row blocks first (at most 64 sequences)
     bool q_aligned, out_aligned; // every row begins at a multiple of 16 bytes
     int64_t q_stride, q_head_stride; // elements
     int64_t o_stride, o_head_stride;
@@ -88,33 +88,77 @@ __device__ __forceinline__ int32_t visibleTokens(const PrefillFp4Args &a, const 
     return n < 0 ? 0 : (n > a.capacity ? a.capacity : n);
 }
 
-// Which (sequence, row block) workgroup x of a KV head works on: the blocks of the last sequence first, each sequence's last
-// block first (it sees the most). False for a workgroup beyond the last block.
-__device__ __forceinline__ bool findBlock(const PrefillFp4Args &a, int lane, int block_rows, int x, int &seq, int &block, Span &span_out) {
+// Which (sequence, row block) workgroup x of a KV head works on. False for a workgroup beyond the last block.
+struct Found {
+    int seq, block;
+    Span span;
+    __device__ __forceinline__ void take(const Span &of_lane, int lane) {
+        span.q_start = __builtin_amdgcn_readlane(of_lane.q_start, lane);
+        span.q_len = __builtin_amdgcn_readlane(of_lane.q_len, lane);
+        span.history = __builtin_amdgcn_readlane(of_lane.history, lane);
+    }
+};
+template <int BM>
+__device__ __forceinline__ int blocksOf(const PrefillFp4Args &a, const Span &s) {
+    const int64_t rows = static_cast<int64_t>(s.q_len) * a.group;
+    return rows > 0 ? static_cast<int>((rows + BM - 1) / BM) : 0;
+}
+// The blocks of the last sequence first, each sequence's last block first (it sees the most).
+template <int BM>
+__device__ __forceinline__ bool findInOrder(const PrefillFp4Args &a, int lane, int x, Found &found) {
     for (int base = 0; base < a.num_seqs; base += 64) {
         const int s = a.num_seqs - 1 - (base + lane);
-        int blocks = 0;
         Span span{0, 0, 0};
         if (s >= 0) {
             span = loadSpan(a, s);
-            const int64_t rows = static_cast<int64_t>(span.q_len) * a.group;
-            blocks = rows > 0 ? static_cast<int>((rows + block_rows - 1) / block_rows) : 0;
         }
-        const int sum = waveInclusiveSum(blocks);
+        const int sum = waveInclusiveSum(blocksOf<BM>(a, span));
         const int all = __builtin_amdgcn_readlane(sum, 63);
         if (x >= all) {
             x -= all;
             continue;
         }
         const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > x));
-        seq = a.num_seqs - 1 - (base + at);
-        block = __builtin_amdgcn_readlane(sum, at) - 1 - x;
-        span_out.q_start = __builtin_amdgcn_readlane(span.q_start, at);
-        span_out.q_len = __builtin_amdgcn_readlane(span.q_len, at);
-        span_out.history = __builtin_amdgcn_readlane(span.history, at);
+        found.seq = a.num_seqs - 1 - (base + at);
+        found.block = __builtin_amdgcn_readlane(sum, at) - 1 - x;
+        found.take(span, at);
         return true;
     }
     return false;
+}
+// Up to 64 sequences, a lane each: the x-th longest block, in steps of 64 tokens. The number of a sequence's blocks that have
+// `steps` steps or more follows from its span (the later a block, the more it sees), so each wavefront bisects for the length.
+template <int BM>
+__device__ __forceinline__ bool findByLength(const PrefillFp4Args &a, int lane, int x, Found &found) {
+    Span span{0, 0, 0};
+    if (lane < a.num_seqs) {
+        span = loadSpan(a, lane);
+    }
+    const int blocks = blocksOf<BM>(a, span);
+    auto atLeast = [&](int steps) { // of this lane's blocks; steps >= 1: those whose last row sees 64 (steps - 1) + 1 tokens
+        const int64_t j = 64 * (static_cast<int64_t>(steps) - 1) - span.history; // the first new token that does
+        if (blocks == 0 || j >= span.q_len || 64 * (steps - 1) >= a.capacity) {
+            return 0;
+        }
+        return j <= 0 ? blocks : blocks - static_cast<int>(j * a.group / BM);
+    };
+    auto sumOf = [](int n) { return __builtin_amdgcn_readlane(waveInclusiveSum(n), 63); };
+    if (x >= sumOf(blocks)) {
+        return false;
+    }
+    const int most = blocks > 0 ? (visibleTokens(a, span, span.q_len - 1) + 63) / 64 : 0;
+    int low = 0, high = __builtin_amdgcn_readfirstlane(waveMaxInt(most)) + 1; // more than x blocks have `low` steps, not `high`
+    while (high - low > 1) {
+        const int middle = (low + high) / 2;
+        (sumOf(atLeast(middle)) > x ? low : high) = middle;
+    }
+    const int longer = atLeast(high), alike = (low == 0 ? blocks : atLeast(low)) - longer;
+    const int before = sumOf(longer), sum = waveInclusiveSum(alike);
+    const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(sum > x - before));
+    found.seq = at;
+    found.block = __builtin_amdgcn_readlane(blocks - longer - alike + sum, at) - 1 - (x - before);
+    found.take(span, at);
+    return true;
 }
 
 // A head's rows in LDS and in the lanes that fill it. K: a lane has 16 bytes of codes, 32 elements under one scale. V: a unit is
@@ -145,15 +189,17 @@ struct Rows {
 };
 
 constexpr int kStep = 64, kTiles = kStep / kTile; // tokens per step
-template <int HEAD>
-constexpr int kPerUnit = HEAD < 256 ? 2 : 1; // workgroups that share a compute unit (its LDS, at head 256)
+// Steps that some rows of a block see in part: what its BM rows see differs by less than BM tokens.
+template <int BM>
+constexpr int kTailSteps = BM / 64 + 1;
 
 // WHOLE: the page size is a multiple of 16, so that a tile lies in one page; otherwise every lane looks its rows up.
-template <typename T, int HEAD, int R, bool WHOLE>
-__global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Kernel(PrefillFp4Args a) {
+// WAVES: 4, or 8 where a tile takes two passes of 64 lanes. Two wavefronts share a SIMD.
+template <typename T, int HEAD, int R, int WAVES, bool WHOLE>
+__global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args a) {
     using S = typename T::storage;
     using G = Rows<HEAD>;
-    constexpr int BM = 64 * R, BN = kStep, TT = kTiles;
+    constexpr int BM = 16 * R * WAVES, BN = kStep, TT = kTiles;
     constexpr int kTileSlots = kTile * G::kChunks;
     struct Tiles {
         uint4 k[2][BN * G::kGroups];         // codes
@@ -161,19 +207,20 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
         uint4 v[2][TT * kTileSlots];         // fp16
     };
     __shared__ Tiles tiles;
-    // values that are not finite: bit t of [step % 3][scale group] = token t of the step
-    __shared__ unsigned long long bad[3][G::kGroups];
-    __shared__ int any_bad[3];
+    // values that are not finite, of the steps that some row does not see to the end: bit t of [step][scale group] = token t
+    __shared__ unsigned long long bad[kTailSteps<BM>][G::kGroups];
 
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kv_head = blockIdx.x % a.num_kv_heads;
 
-    int seq, block;
-    Span span;
-    if (!findBlock(a, lane, BM, blockIdx.x / a.num_kv_heads, seq, block, span)) {
+    Found found;
+    const int x = blockIdx.x / a.num_kv_heads;
+    if (a.by_length ? !findByLength<BM>(a, lane, x, found) : !findInOrder<BM>(a, lane, x, found)) {
         return;
     }
+    const int seq = found.seq, block = found.block;
+    const Span span = found.span;
     const int total_rows = span.q_len * a.group;
     const int block_row0 = block * BM;
     const int last_row = min(block_row0 + BM, total_rows) - 1;
@@ -182,12 +229,11 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
         return;
     }
     const int n_steps = (block_visible + BN - 1) / BN;
+    // steps that every row of the block sees to the end
+    const int full_steps = __builtin_amdgcn_readfirstlane(visibleTokens(a, span, block_row0 / a.group)) / BN;
 
-    if (threadIdx.x < 3 * G::kGroups) {
+    if (threadIdx.x < kTailSteps<BM> * G::kGroups) {
         (&bad[0][0])[threadIdx.x] = 0;
-    }
-    if (threadIdx.x < 3) {
-        any_bad[threadIdx.x] = 0;
     }
 
     // ---- this lane's columns: row c of each of the wavefront's R groups of 16 rows ----
@@ -252,57 +298,76 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
     most_visible = __builtin_amdgcn_readfirstlane(waveMaxInt(most_visible));
     least_visible = __builtin_amdgcn_readfirstlane(-waveMaxInt(-least_visible));
 
-    // ---- loads: codes and scales of this wavefront's tile of a step ----
-    const int own_tile = w;
+    // ---- loads: codes and scales of this wavefront's tile of a step (WAVES = 8: of one pass over it) ----
+    constexpr int kWavesPerTile = WAVES / kTiles;
+    constexpr int kPassesK = G::kPassesK / kWavesPerTile, kPasses = G::kPasses / kWavesPerTile;
+    static_assert(kWavesPerTile == 1 || (G::kPassesK == 2 && G::kPasses == 2), "a pass for each wavefront of a tile");
+    const int own_tile = w / kWavesPerTile, in_tile = 64 * (w % kWavesPerTile) + lane; // the lane's place in the first pass
     const int64_t table_row = seq * a.block_table_stride;
     const int last_entry = (block_visible - 1) / a.block_size;
     auto entryId = [&](int entry) { return clampPage(loadIndexOf(a.index_type, a.block_tables, table_row + min(entry, last_entry)), a.num_blocks); };
 
     struct Raw { // what a lane has loaded, per pass
-        uint32_t k[G::kPassesK][4], v[G::kPasses][G::kUnitWords];
-        uint32_t ks[G::kPassesK], vs[G::kPasses];
+        uint32_t k[kPassesK][4], v[kPasses][G::kUnitWords];
+        uint32_t ks[kPassesK], vs[kPasses];
     };
     Raw raw;
     // which row of the tile and which chunk or unit of it this lane has: K chunk-fastest (contiguous loads), V token-fastest
     // (see vSlot)
-    auto kRow = [&](int p) { return (64 * p + lane) / G::kGroups; };
-    auto kChunkOf = [&](int p) { return (64 * p + lane) % G::kGroups; };
-    auto hasK = [&](int p) { return 64 * p + lane < kTile * G::kGroups; };
+    auto kRow = [&](int p) { return (64 * p + in_tile) / G::kGroups; };
+    auto kChunkOf = [&](int p) { return (64 * p + in_tile) % G::kGroups; };
+    auto hasK = [&](int p) { return 64 * p + in_tile < kTile * G::kGroups; };
     auto vRow = [&](int p) { return lane & 15; };
-    auto vUnitOf = [&](int p) { return (64 * p + lane) >> 4; };
-    auto hasV = [&](int p) { return 64 * p + lane < kTile * G::kUnits; };
+    auto vUnitOf = [&](int p) { return (64 * p + in_tile) >> 4; };
+    auto hasV = [&](int p) { return 64 * p + in_tile < kTile * G::kUnits; };
 
-    // table entries of 64 pages, a batch ahead (WHOLE)
+    // Where the tile lies that is loaded next. WHOLE: table entries of 64 pages in the lanes, and the 64 behind them; its entry
+    // and row there. Otherwise: page and row of each of its tokens (lane & 15), looked up a step ahead.
+    int t_next = kTile * own_tile;
     int batch = 0, ids = 0, ids_next = 0;
-    int entry = kTile * own_tile / a.block_size, row_in_page = kTile * own_tile - entry * a.block_size; // of the tile that comes next
+    int entry = 0, row_in_page = 0;
+    auto lookUp = [&]() {
+        const int token = min(t_next + (lane & 15), block_visible - 1);
+        entry = token / a.block_size;
+        row_in_page = token - entry * a.block_size;
+        ids = entryId(entry);
+    };
     if constexpr (WHOLE) {
+        entry = t_next / a.block_size;
+        row_in_page = t_next - entry * a.block_size;
         ids = entryId(lane);
         ids_next = entryId(64 + lane);
+    } else {
+        lookUp();
     }
-    auto load = [&](int step) {
-        const int t = step * BN + kTile * own_tile;
+    // before load(): the entry of the tile that comes next is at hand
+    auto turnPages = [&]() {
         if constexpr (WHOLE) {
-            if (t < block_visible) {
-                while (row_in_page >= a.block_size) {
-                    row_in_page -= a.block_size;
-                    ++entry;
-                }
-            } else { // behind what the block sees: the last tile that it does, again
-                entry = last_entry;
-                row_in_page = (block_visible - 1) / kTile * kTile - entry * a.block_size;
-            }
-            const int e = entry, row0 = row_in_page;
-            row_in_page += BN;
-            if ((e >> 6) > batch) {
+            if ((entry >> 6) > batch && t_next < block_visible) {
                 ++batch;
                 ids = ids_next;
                 ids_next = entryId(64 * (batch + 1) + lane);
             }
+        }
+    };
+    // The tiles come in order, 64 tokens apart; behind what the block sees, the last one that it does, again.
+    auto load = [&]() {
+        if constexpr (WHOLE) {
+            const bool inside = t_next < block_visible;
+            const int e = inside ? entry : last_entry, row0 = inside ? row_in_page : (block_visible - 1) / kTile * kTile - last_entry * a.block_size;
             const int64_t id = __builtin_amdgcn_readlane(ids, e & 63);
+            t_next += BN;
+            row_in_page += BN;
+#pragma unroll
+            for (int i = 0; i < BN / 16; ++i) { // (pages of 16 tokens or more)
+                const bool over = row_in_page >= a.block_size;
+                row_in_page -= over ? a.block_size : 0;
+                entry += over ? 1 : 0;
+            }
             auto tile = [&](const PoolSide &s) { return s.base + id * s.block + kv_head * s.head + static_cast<int64_t>(row0) * s.row; };
             const char *k_codes = tile(a.k_codes), *k_scales = tile(a.k_scales);
 #pragma unroll
-            for (int p = 0; p < G::kPassesK; ++p) {
+            for (int p = 0; p < kPassesK; ++p) {
                 if (hasK(p)) {
                     loadWords<16, false>(k_codes + kRow(p) * a.k_codes.row + 16 * kChunkOf(p), raw.k[p]);
                     raw.ks[p] = static_cast<uint8_t>(k_scales[kRow(p) * a.k_scales.row + kChunkOf(p)]);
@@ -310,41 +375,43 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
             }
             const char *v_codes = tile(a.v_codes), *v_scales = tile(a.v_scales);
 #pragma unroll
-            for (int p = 0; p < G::kPasses; ++p) {
+            for (int p = 0; p < kPasses; ++p) {
                 if (hasV(p)) {
                     loadWords<4 * G::kUnitWords, false>(v_codes + vRow(p) * a.v_codes.row + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
                     raw.vs[p] = static_cast<uint8_t>(v_scales[vRow(p) * a.v_scales.row + vUnitOf(p) * G::kUnit / 32]);
                 }
             }
         } else {
-            auto rowOf = [&](const PoolSide &s, int64_t id, int row) { return s.base + id * s.block + kv_head * s.head + static_cast<int64_t>(row) * s.row; };
+            auto rowOf = [&](const PoolSide &s, int id, int row) { return s.base + id * s.block + kv_head * s.head + static_cast<int64_t>(row) * s.row; };
 #pragma unroll
-            for (int p = 0; p < G::kPassesK; ++p) {
+            for (int p = 0; p < kPassesK; ++p) {
+                const int id = __shfl(ids, kRow(p) & 15, 64), row = __shfl(row_in_page, kRow(p) & 15, 64);
                 if (hasK(p)) {
-                    const int token = min(t + kRow(p), block_visible - 1), e = token / a.block_size;
-                    const int id = entryId(e), row = token - e * a.block_size;
                     loadWords<16, false>(rowOf(a.k_codes, id, row) + 16 * kChunkOf(p), raw.k[p]);
                     raw.ks[p] = static_cast<uint8_t>(rowOf(a.k_scales, id, row)[kChunkOf(p)]);
                 }
             }
 #pragma unroll
-            for (int p = 0; p < G::kPasses; ++p) {
-                if (hasV(p)) {
-                    const int token = min(t + vRow(p), block_visible - 1), e = token / a.block_size;
-                    const int id = entryId(e), row = token - e * a.block_size;
-                    loadWords<4 * G::kUnitWords, false>(rowOf(a.v_codes, id, row) + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
-                    raw.vs[p] = static_cast<uint8_t>(rowOf(a.v_scales, id, row)[vUnitOf(p) * G::kUnit / 32]);
+            for (int p = 0; p < kPasses; ++p) {
+                if (hasV(p)) { // (vRow is the lane's own token)
+                    loadWords<4 * G::kUnitWords, false>(rowOf(a.v_codes, ids, row_in_page) + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
+                    raw.vs[p] = static_cast<uint8_t>(rowOf(a.v_scales, ids, row_in_page)[vUnitOf(p) * G::kUnit / 32]);
                 }
             }
+            t_next += BN;
+            lookUp();
         }
     };
-    // What was loaded for `step`, in LDS: K as it is, V as 16-bit values. Rows that nobody of the block sees (behind the
-    // sequence's end, or behind the block's last row) may hold anything: their scores are masked, their values go in as zeros.
-    auto convert = [&](int step) {
+    // What was loaded for `step`, in LDS: K as it is, V as 16-bit values. Where all rows see all of the step (FULL), a value that
+    // is not finite goes in as the NaN that it gives to all of them. Elsewhere it goes in as zero, and is noted; rows that nobody
+    // of the block sees (behind the sequence's end, or behind the block's last row) may hold anything: their scores are masked,
+    // their values go in as zeros.
+    auto convert = [&](int step, auto full) {
+        constexpr bool FULL = decltype(full)::value;
         uint4 *k_to = tiles.k[step & 1] + own_tile * (kTile * G::kGroups);
         uint8_t *scales_to = reinterpret_cast<uint8_t *>(tiles.k_scales[step & 1]) + own_tile;
 #pragma unroll
-        for (int p = 0; p < G::kPassesK; ++p) {
+        for (int p = 0; p < kPassesK; ++p) {
             if (hasK(p)) {
                 k_to[G::K::kSlot(kRow(p), kChunkOf(p))] = make_uint4(raw.k[p][0], raw.k[p][1], raw.k[p][2], raw.k[p][3]);
                 scales_to[4 * (kTile * kChunkOf(p) + kRow(p))] = static_cast<uint8_t>(raw.ks[p]);
@@ -353,18 +420,17 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
         uint4 *to = tiles.v[step & 1] + own_tile * kTileSlots;
         const int t = kTile * own_tile;
 #pragma unroll
-        for (int p = 0; p < G::kPasses; ++p) {
+        for (int p = 0; p < kPasses; ++p) {
             if (hasV(p)) {
-                const bool seen = step * BN + t + vRow(p) < block_visible;
-                const bool finite = raw.vs[p] != 0xff;
-                const float scale = seen && finite ? mx::scaleOf(raw.vs[p]) : 0.0f;
+                const bool seen = FULL || step * BN + t + vRow(p) < block_visible;
+                const bool zero = !FULL && raw.vs[p] == 0xff;
+                const float scale = seen && !(zero && step >= full_steps) ? mx::scaleOf(raw.vs[p]) : 0.0f;
 #pragma unroll
                 for (int i = 0; i < G::kUnitWords; ++i) {
                     to[G::vSlot(vRow(p), G::kUnitWords * vUnitOf(p) + i)] = mx::toF16x8(raw.v[p][i], scale);
                 }
-                if (seen && !finite) {
-                    atomicOr(&bad[step % 3][vUnitOf(p) * G::kUnit / 32], 1ull << (t + vRow(p)));
-                    any_bad[step % 3] = 1;
+                if (seen && zero && step >= full_steps) {
+                    atomicOr(&bad[step - full_steps][vUnitOf(p) * G::kUnit / 32], 1ull << (t + vRow(p)));
                 }
             }
         }
@@ -384,8 +450,8 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
         m[r] = -INFINITY;
         shift[r] = 0.0f;
     }
-    const bool plain = a.alibi_slopes == nullptr && a.scale_log2 > 0.0f;
-    const float unit = plain ? a.scale_log2 : 1.0f;
+    const bool plain_call = a.alibi_slopes == nullptr && a.scale_log2 > 0.0f;
+    const float unit = plain_call ? a.scale_log2 : 1.0f;
     const float lazy = kLazyLog2 / unit;
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 *LdsPiece;
@@ -395,7 +461,8 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
     const uint32_t one2 = TileF16::pack2(1.0f, 1.0f);
     const uint4 ones = make_uint4(one2, one2, one2, one2);
 
-    auto compute = [&](int step, auto between) {
+    auto compute = [&](int step, auto plain, auto full, auto between) {
+        constexpr bool PLAIN = decltype(plain)::value, FULL = decltype(full)::value;
         const int buf = step & 1, t0 = step * BN;
         f32x4 s[R][TT];
         uint32_t k_scales[G::kSets];
@@ -423,10 +490,11 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
             }
         }
         between();
-        uint4 p_op[R][TT / 2];
+        float top[R];
+        bool above = false;
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            if (!plain) {
+            if constexpr (!PLAIN) {
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
@@ -435,7 +503,7 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
                     }
                 }
             }
-            if (t0 + BN > least_visible) {
+            if (!FULL && t0 + BN > least_visible) {
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
@@ -444,15 +512,19 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
                     }
                 }
             }
-            float top = maxOf(s[r][0][0], s[r][0][1]); // (three-operand maxima)
+            top[r] = maxOf(s[r][0][0], s[r][0][1]); // (three-operand maxima)
 #pragma unroll
             for (int j = 2; j < 4 * TT; j += 2) {
-                top = maxOf(maxOf(top, s[r][j / 4][j % 4]), s[r][j / 4][j % 4 + 1]);
+                top[r] = maxOf(maxOf(top[r], s[r][j / 4][j % 4]), s[r][j / 4][j % 4 + 1]);
             }
             // (a row that has seen nothing has m = -inf: any finite maximum is above it; a NaN is above nothing, and reaches
             // the outputs by its own probability)
-            if (__builtin_amdgcn_ballot_w64(top > m[r] + lazy) != 0) {
-                const float m_new = maxOf(m[r], maxAcrossTokenGroups(top));
+            above |= top[r] > m[r] + lazy;
+        }
+        if (__builtin_amdgcn_ballot_w64(above) != 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float m_new = maxOf(m[r], maxAcrossTokenGroups(top[r]));
                 const float alpha = m_new > m[r] ? fastExp2((m[r] - m_new) * unit) : 1.0f;
                 m[r] = m_new;
                 shift[r] = m_new == -INFINITY ? 0.0f : -m_new * unit;
@@ -462,6 +534,10 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
                     o[r][e] *= alpha;
                 }
             }
+        }
+        uint4 p_op[R][TT / 2];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
 #pragma unroll
             for (int u = 0; u < TT / 2; ++u) {
                 uint32_t words[4];
@@ -492,14 +568,14 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
                 }
             }
         }
-        if (any_bad[step % 3] != 0) {
+        if (!FULL && step >= full_steps) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const int n = visible[r] - t0;
                 const unsigned long long sees = n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1);
 #pragma unroll
                 for (int e = 0; e < G::kCols; ++e) {
-                    if ((bad[step % 3][e / 2] & sees) != 0) {
+                    if ((bad[step - full_steps][e / 2] & sees) != 0) {
                         o[r][e] = f32x4{NAN, NAN, NAN, NAN};
                     }
                 }
@@ -508,37 +584,48 @@ __global__ void __launch_bounds__(kPrefillThreads, kPerUnit<HEAD>) prefillFp4Ker
     };
 
     // ---- pipeline: codes two steps ahead in registers, values one step ahead in LDS ----
-    load(0);
+    turnPages();
+    load();
     __syncthreads(); // the notes of values that are not finite are clear
-    convert(0);
-    if (n_steps > 1) {
-        load(1);
-    }
+    convert(0, std::false_type{});
+    turnPages();
+    load();
     __syncthreads();
-    for (int step = 0; step < n_steps; ++step) {
-        if (threadIdx.x < G::kGroups) { // of step - 1, read before the last barrier, for step + 2
-            bad[(step + 2) % 3][threadIdx.x] = 0;
-            any_bad[(step + 2) % 3] = 0;
+    auto walk = [&](auto plain) {
+        int step = 0;
+        for (; step + 1 < full_steps; ++step) { // nothing to decide: one run of instructions up to the row maxima
+            turnPages();
+            compute(step, plain, std::true_type{}, [&]() {
+                convert(step + 1, std::true_type{});
+                load();
+            });
+            __syncthreads();
         }
-        auto next = [&]() {
-            if (step + 1 < n_steps) {
-                convert(step + 1);
-                if (step + 2 < n_steps) {
-                    load(step + 2);
+        for (; step < n_steps; ++step) {
+            auto next = [&]() {
+                if (step + 1 < n_steps) {
+                    convert(step + 1, std::false_type{});
+                    turnPages();
+                    load();
                 }
+            };
+            if (step * BN < most_visible) {
+                compute(step, plain, std::false_type{}, next);
+            } else { // nothing that this wavefront's rows see
+                next();
             }
-        };
-        if (step * BN < most_visible) {
-            compute(step, next);
-        } else { // nothing that this wavefront's rows see
-            next();
+            __syncthreads();
         }
-        __syncthreads();
+    };
+    if (plain_call) {
+        walk(std::true_type{});
+    } else {
+        walk(std::false_type{});
     }
 
     // ---- normalise and store: a lane holds four consecutive columns of row c of a group; the wavefront's rows pass through
     // LDS (nobody reads the tiles any more) and leave as 16-byte pieces ----
-    static_assert(sizeof(Tiles) >= 4 * R * 16 * HEAD * 2, "the tiles hold the output rows of all four wavefronts");
+    static_assert(sizeof(Tiles) >= BM * HEAD * 2, "the tiles hold the output rows of all wavefronts");
     auto piece = [](int row, int chunk) { return row * G::kChunks + (chunk ^ (row & (G::kSwizzle - 1))); };
     uint4 *stage = reinterpret_cast<uint4 *>(&tiles) + w * (R * 16 * G::kChunks);
 #pragma unroll
