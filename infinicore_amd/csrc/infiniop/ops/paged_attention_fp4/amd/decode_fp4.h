@@ -23,10 +23,10 @@
 //
 // Work is dealt in one of two ways (wholeSequences in decode_fp4_launch.h has the times on both sides):
 //   * whole: a workgroup of eight wavefronts for a sequence and KV head, joined in LDS;
-//   * by runs: the steps of all sequences, one after the other, are cut into as many equal runs as there are wavefronts for a KV
-//     head. A run may hold the end of one sequence, whole ones, and the start of another; whole sequences are normalised and
-//     written at once, the others leave accumulators, reference points and denominators, which the merge kernel joins in the
-//     order of the runs.
+//   * by runs: the steps of all sequences, one after the other, are cut into as many equal runs as there are workgroups (of four
+//     wavefronts) for a KV head. A run may hold the end of one sequence, whole ones, and the start of another; the wavefronts
+//     share the steps of each and join in LDS; whole sequences are normalised and written at once, the others leave
+//     accumulators, reference points and denominators, which the merge kernel joins in the order of the runs.
 // RUNS (runs of a few query tokens per sequence, for prefill): rows are (query token, head) pairs, 16 to a segment, each with
 // the tokens that it sees.
 #ifndef INFINICORE_AMD_PA_DECODE_FP4_H
@@ -54,9 +54,9 @@ using op::paged_attention::amd::waveMaxInt;
 namespace mx = device::amd::mx;
 
 constexpr int kStepTokens = 32;
-constexpr int kDecodeThreads = 256;  // four wavefronts that share nothing but the launch
+constexpr int kDecodeThreads = 256;
 constexpr int kWholeThreads = 512;
-constexpr int kLeastSteps = 1;       // of a run
+constexpr int kLeastSteps = 4;       // of a run: one for each of its wavefronts
 constexpr float kLazyLog2 = 8.0f;    // how far (in powers of two) a maximum may outgrow its reference point
 
 enum class IndexType : int32_t { i64, i32, u32 };
@@ -735,49 +735,80 @@ __device__ __forceinline__ void storeColumns(typename T::storage *to, const floa
     }
 }
 
-// What the lanes hold of a segment: normalised outputs (`whole`), or a partial result at place `place`.
-template <typename T, int HEAD, bool RUNS>
-__device__ __forceinline__ void finish(const DecodeState<T, HEAD> &st, const Rows &rows, bool whole, int64_t place, int kv_head,
-                                       int segment, int first_token, int q_len, int lane) {
+// From nothing.
+template <typename T, int HEAD>
+__device__ __forceinline__ void clear(DecodeState<T, HEAD> &st) {
+    st.m = -INFINITY;
+    st.shift = 0.0f;
+    st.l = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < HEAD / 16; ++e) {
+        st.o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+}
+
+// What the wavefronts of a workgroup hold of a segment, side by side in LDS, where their steps were.
+template <int HEAD, int WAVES>
+struct Joined {
+    float acc[WAVES][kHeadsPerWave][HEAD];
+    float2 ml[WAVES][kHeadsPerWave]; // reference point (log2), denominator
+};
+// The wavefront's own, of the segment's first `count` rows.
+template <typename T, int HEAD, int WAVES>
+__device__ __forceinline__ void leave(Joined<HEAD, WAVES> &to, const DecodeState<T, HEAD> &st, float unit, int wave, int lane, int count) {
     using L = Layout<HEAD>;
-    const ArgsAgain a = argsAgain();
     const int g = lane >> 4, c = lane & 15;
-    const int part_rows = a->part_rows;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = 4 * g + i;
         const float m = __shfl(st.m, r, 64);
-        const int visible = RUNS ? __shfl(rows.visible, r, 64) : 1;
-        const RowPlace at = rowPlace<RUNS>(a->group, kv_head, segment, r, first_token, q_len);
-        if (!at.exists || visible <= 0) {
-            continue;
-        }
-        const float f = whole ? 1.0f / st.l[i] : 1.0f;
-        float x[L::kCols];
-#pragma unroll
-        for (int e = 0; e < L::kCols; ++e) {
-            x[e] = st.o[e][i] * f;
-        }
-        if (whole) {
-            auto *row = static_cast<typename T::storage *>(a->out) + at.token * a->o_stride + at.head * a->o_head_stride;
-            const bool aligned = a->out_aligned;
-            storeColumns<T, L::kStripCols>(row + L::column(0, c), x, aligned);
-            if constexpr (L::kStrips > 1) {
-                storeColumns<T, 4>(row + L::column(1, c), x + L::kStripCols, aligned);
-            }
-        } else {
+        if (r < count) {
             if (c == 0) {
-                a->part_ml[place * part_rows + r] = make_float2(m * rows.unit, st.l[i]);
+                to.ml[wave][r] = make_float2(m * unit, st.l[i]);
             }
-            float *row = a->part_acc + (place * part_rows + r) * HEAD;
 #pragma unroll
             for (int e = 0; e < L::kCols; e += 4) {
                 const int strip = e < L::kStripCols ? 0 : 1;
-                float *to = row + L::column(strip, c) + (strip == 0 ? e : e - L::kStripCols);
-                *reinterpret_cast<float4 *>(to) = make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+                *reinterpret_cast<float4 *>(&to.acc[wave][r][L::column(strip, c) + (strip == 0 ? e : e - L::kStripCols)]) =
+                    make_float4(st.o[e][i], st.o[e + 1][i], st.o[e + 2][i], st.o[e + 3][i]);
             }
         }
     }
+}
+// Joined in the order of the wavefronts, four columns of a row a thread: put(row, column, reference point, denominator, sums).
+template <int HEAD, int WAVES, typename Put>
+__device__ __forceinline__ void join(const Joined<HEAD, WAVES> &from, int count, const Put &put) {
+    constexpr int kLanes = HEAD / 4;
+    for (int at = threadIdx.x; at < count * kLanes; at += 64 * WAVES) {
+        const int r = at / kLanes, column = 4 * (at % kLanes);
+        float m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            m = maxOf(m, from.ml[w][r].x);
+        }
+        float l = 0.0f;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float2 ml = from.ml[w][r];
+            const float f = ml.x == m ? 1.0f : fastExp2(ml.x - m);
+            const float4 v = *reinterpret_cast<const float4 *>(&from.acc[w][r][column]);
+            l += ml.y * f;
+            x.x += v.x * f;
+            x.y += v.y * f;
+            x.z += v.z * f;
+            x.w += v.w * f;
+        }
+        put(r, column, m, l, x);
+    }
+}
+// Four columns of an output row, normalised.
+template <typename T>
+__device__ __forceinline__ void storeOutput(ArgsAgain a, const RowPlace &at, int column, float l, float4 x) {
+    const float f = 1.0f / l;
+    const float y[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
+    auto *row = static_cast<typename T::storage *>(a->out) + at.token * a->o_stride + at.head * a->o_head_stride;
+    storeColumns<T, 4>(row + column, y, a->out_aligned);
 }
 
 // Steps [from, to) of a segment, from nothing: what the lanes hold afterwards is theirs alone.
@@ -814,13 +845,7 @@ __device__ __forceinline__ void walk(Pages<HEAD, GRAIN> &pages, Step<HEAD> (&rin
         asm volatile("" : "+v"(st.q[w].x), "+v"(st.q[w].y), "+v"(st.q[w].z), "+v"(st.q[w].w));
     }
     asm volatile("" : "+v"(rows.slope_log2));
-    st.m = -INFINITY;
-    st.shift = 0.0f;
-    st.l = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int e = 0; e < HEAD / 16; ++e) {
-        st.o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    clear(st);
     int stage = 0;
     for (int step = from; step < to; ++step) {
         // the loads of this step are done; those of the steps behind it, up to kStages - 1, may be under way
@@ -842,13 +867,19 @@ __device__ __forceinline__ void walk(Pages<HEAD, GRAIN> &pages, Step<HEAD> (&rin
     }
 }
 
-// Grid: KV heads x (runs / 4) x chunks of heads. Two neighbouring KV heads take turns on the dies: their scales share cache
+// A workgroup's run: its four wavefronts share the steps of each segment in it and join what they have in LDS. Grid: KV heads x
+// runs x chunks of heads. Two neighbouring KV heads take turns on the dies: their scales share cache
 // lines, and a die that works on both at a time fetches them once.
 template <typename T, int HEAD, int GRAIN, bool RUNS>
 __global__ void __launch_bounds__(kDecodeThreads, Layout<HEAD>::kPerUnit)
 decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_type_, int32_t num_seqs, int32_t capacity, int32_t most_runs,
                 DecodeFp4Args a) {
-    __shared__ Step<HEAD> rings[kDecodeThreads / 64][Layout<HEAD>::kStages];
+    constexpr int kWaves = kDecodeThreads / 64;
+    __shared__ union Shared {
+        Step<HEAD> rings[kWaves][Layout<HEAD>::kStages];
+        Joined<HEAD, kWaves> joined;
+        __device__ Shared() {}
+    } shared;
     const IndexType index_type = static_cast<IndexType>(index_type_);
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -866,7 +897,7 @@ decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_ty
     }
     const bool paired = (gridDim.x & 1) == 0 && (gridDim.y & 1) == 0;
     const int kv_head = paired ? (blockIdx.x & ~1u) | (blockIdx.y & 1) : blockIdx.x;
-    const uint32_t run = 4 * (paired ? (blockIdx.y & ~1u) | (blockIdx.x & 1) : blockIdx.y) + wave;
+    const uint32_t run = paired ? (blockIdx.y & ~1u) | (blockIdx.x & 1) : blockIdx.y;
     const int chunk = blockIdx.z;
     const uint32_t runs = runsFor(most_runs, total);
     if (RUNS && blockIdx.x + blockIdx.y == 0 && threadIdx.x == 0 && a.num_segments != nullptr) {
@@ -879,7 +910,6 @@ decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_ty
     uint32_t at = cut.start(run);
     const uint32_t end = cut.start(run + 1);
 
-    auto &ring = rings[wave];
     Pages<HEAD, GRAIN> pages(a, lane, kv_head);
     DecodeState<T, HEAD> st;
     Rows rows(a);
@@ -914,16 +944,40 @@ decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_ty
             const int from = static_cast<int>(at - start);
             const int to = static_cast<int>(end - start < static_cast<uint32_t>(steps) ? end - start : steps);
 
-            walk<T, HEAD, GRAIN, RUNS>(pages, ring, st, rows, lane, kv_head, seq, segment, tokens, first_token, q_len, history, from, to);
+            const Cut share(static_cast<uint32_t>(to - from), kWaves);
+            const int mine_from = from + static_cast<int>(share.start(wave)), mine_to = from + static_cast<int>(share.start(wave + 1));
+            if (mine_from < mine_to) {
+                walk<T, HEAD, GRAIN, RUNS>(pages, shared.rings[wave], st, rows, lane, kv_head, seq, segment, tokens, first_token, q_len,
+                                           history, mine_from, mine_to);
+            } else {
+                clear(st);
+            }
+            const ArgsAgain again = argsAgain();
+            const int group = again->group;
+            const int count = min((RUNS ? q_len * group : group) - segment * kHeadsPerWave, kHeadsPerWave);
+            __syncthreads(); // the steps are not read any more
+            leave<T>(shared.joined, st, rows.unit, wave, lane, count);
+            __syncthreads();
             const bool whole = from == 0 && to == steps;
-            if (from == 0) {
-                const ArgsAgain again = argsAgain();
-                if (again->segments != nullptr && kv_head + chunk == 0 && lane == 0) { // the same in every stream
-                    again->segments[id] = make_int4(run, cut.runOf(start + steps - 1), seq, segment);
-                }
+            if (from == 0 && again->segments != nullptr && kv_head + chunk == 0 && threadIdx.x == 0) { // the same in every stream
+                again->segments[id] = make_int4(run, cut.runOf(start + steps - 1), seq, segment);
             }
             const int64_t place = (static_cast<int64_t>(kv_head * static_cast<int>(gridDim.z) + chunk) * most_runs + run) * 2 + (from == 0 ? 1 : 0);
-            finish<T, HEAD, RUNS>(st, rows, whole, place, kv_head, segment, first_token, q_len, lane);
+            join(shared.joined, count, [&](int r, int column, float m, float l, float4 x) {
+                if (whole) {
+                    const RowPlace at_row = rowPlace<RUNS>(group, kv_head, segment, r, first_token, q_len);
+                    if (!RUNS || history + (at_row.token - first_token) + 1 > 0) {
+                        storeOutput<T>(again, at_row, column, l, x);
+                    }
+                } else {
+                    const int64_t part = place * again->part_rows + r;
+                    if (column == 0) {
+                        again->part_ml[part] = make_float2(m, l);
+                    }
+                    *reinterpret_cast<float4 *>(again->part_acc + part * HEAD + column) = x;
+                }
+            });
+            __syncthreads(); // (of the next segment's steps)
             at = start + to;
         }
         before += all;
@@ -937,17 +991,13 @@ template <typename T, int HEAD, int GRAIN>
 __global__ void __launch_bounds__(kWholeThreads, Layout<HEAD>::kWholePerUnit)
 decodeWholeFp4Kernel(const void *seq_lens, const void *, int32_t index_type, int32_t, int32_t capacity, int32_t, DecodeFp4Args a) {
     using L = Layout<HEAD>;
-    constexpr int kWaves = kWholeThreads / 64, kLanes = HEAD / 4;
-    struct Joined { // [wave][row][column]
-        float acc[kWaves][kHeadsPerWave][HEAD];
-        float2 ml[kWaves][kHeadsPerWave];
-    };
+    constexpr int kWaves = kWholeThreads / 64;
     __shared__ union Shared {
         Step<HEAD> rings[kWaves][L::kWholeStages];
-        Joined joined;
+        Joined<HEAD, kWaves> joined;
         __device__ Shared() {}
     } shared;
-    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool paired = (gridDim.x & 1) == 0 && (gridDim.y & 1) == 0;
     const int kv_head = paired ? (blockIdx.x & ~1u) | (blockIdx.y & 1) : blockIdx.x;
@@ -962,62 +1012,19 @@ decodeWholeFp4Kernel(const void *seq_lens, const void *, int32_t index_type, int
     DecodeState<T, HEAD> st;
     Rows rows(a);
     const int from = cut.start(wave), to = cut.start(wave + 1);
-    st.m = -INFINITY; // of a wavefront without steps
     if (from < to) {
         walk<T, HEAD, GRAIN, false>(pages, shared.rings[wave], st, rows, lane, kv_head, seq, chunk, tokens, seq, 1, 0, from, to);
     } else {
-        st.l = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int e = 0; e < L::kCols; ++e) {
-            st.o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        }
+        clear(st);
     }
-    __syncthreads(); // the rings are not read any more
+    __syncthreads(); // the steps are not read any more
     const ArgsAgain again = argsAgain();
     const int group = again->group, heads = min(group - chunk * kHeadsPerWave, kHeadsPerWave);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = 4 * g + i;
-        const float m = __shfl(st.m, r, 64);
-        if (r < heads) {
-            if (c == 0) {
-                shared.joined.ml[wave][r] = make_float2(m * rows.unit, st.l[i]);
-            }
-#pragma unroll
-            for (int e = 0; e < L::kCols; e += 4) {
-                const int strip = e < L::kStripCols ? 0 : 1;
-                *reinterpret_cast<float4 *>(&shared.joined.acc[wave][r][L::column(strip, c) + (strip == 0 ? e : e - L::kStripCols)]) =
-                    make_float4(st.o[e][i], st.o[e + 1][i], st.o[e + 2][i], st.o[e + 3][i]);
-            }
-        }
-    }
+    leave<T>(shared.joined, st, rows.unit, wave, lane, heads);
     __syncthreads();
-    for (int at = threadIdx.x; at < heads * kLanes; at += kWholeThreads) {
-        const int r = at / kLanes, column = 4 * (at % kLanes);
-        float m = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            m = maxOf(m, shared.joined.ml[w][r].x);
-        }
-        float l = 0.0f;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float2 ml = shared.joined.ml[w][r];
-            const float f = ml.x == m ? 1.0f : fastExp2(ml.x - m);
-            const float4 v = *reinterpret_cast<const float4 *>(&shared.joined.acc[w][r][column]);
-            l += ml.y * f;
-            x.x += v.x * f;
-            x.y += v.y * f;
-            x.z += v.z * f;
-            x.w += v.w * f;
-        }
-        const float f = 1.0f / l;
-        const float y[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
-        auto *row = static_cast<typename T::storage *>(again->out) + seq * again->o_stride
-                  + (kv_head * group + chunk * kHeadsPerWave + r) * again->o_head_stride;
-        storeColumns<T, 4>(row + column, y, again->out_aligned);
-    }
+    join(shared.joined, heads, [&](int r, int column, float, float l, float4 x) {
+        storeOutput<T>(again, rowPlace<false>(group, kv_head, chunk, r, seq, 1), column, l, x);
+    });
 }
 
 // The parts of a segment that lies in more than one run, joined: a workgroup per (segment, row, stream). A quarter of the

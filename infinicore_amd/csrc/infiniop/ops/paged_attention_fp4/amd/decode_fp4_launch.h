@@ -23,10 +23,9 @@ struct DecodePlan {
     size_t workspaceBytes() const { return runs > 1 ? acc_bytes + ml_bytes + segment_bytes + 256 + 256 : 0; } // (256: to align it here; a count)
 };
 
-// Wavefronts that a compute unit holds at a time: that many runs fill the device once.
-inline int wavesPerUnit(size_t head) {
-    const int groups = head == 64 ? Layout<64>::kPerUnit : head == 128 ? Layout<128>::kPerUnit : head == 192 ? Layout<192>::kPerUnit : Layout<256>::kPerUnit;
-    return groups * (kDecodeThreads / 64);
+// Workgroups that a compute unit holds at a time: that many runs fill the device once.
+inline int groupsPerUnit(size_t head) {
+    return head == 64 ? Layout<64>::kPerUnit : head == 128 ? Layout<128>::kPerUnit : head == 192 ? Layout<192>::kPerUnit : Layout<256>::kPerUnit;
 }
 
 // Whether every sequence is left to one workgroup per KV head (and 16 query heads): no scan of the lengths in front, no partial
@@ -69,7 +68,7 @@ inline DecodePlan planDecode(const AttentionFp4Info &in, bool by_rows, int compu
         return plan;
     }
     const int64_t steps = segments * per_segment;
-    const int64_t fill = (static_cast<int64_t>(compute_units) * wavesPerUnit(in.head_size) + streams - 1) / streams;
+    const int64_t fill = (static_cast<int64_t>(compute_units) * groupsPerUnit(in.head_size) + streams - 1) / streams;
     plan.runs = static_cast<int>(std::max<int64_t>(1, std::min(fill, (steps + kLeastSteps - 1) / kLeastSteps)));
     // wavefronts that join the parts of a row, by how many parts there are if the segments are alike
     const int64_t parts = plan.runs / std::max<int64_t>(segments, 1) + 2;
@@ -140,8 +139,7 @@ inline DecodeFp4Args decodeArgs(const AttentionFp4Info &in, const DecodePlan &pl
 
 template <typename T, int HEAD, int GRAIN, bool RUNS>
 void launchDecode(const DecodeFp4Args &a, const DecodePlan &plan, hipStream_t stream) {
-    constexpr int kWaves = kDecodeThreads / 64;
-    unsigned groups = static_cast<unsigned>((plan.runs + kWaves - 1) / kWaves);
+    unsigned groups = static_cast<unsigned>(plan.runs);
     groups += a.num_kv_heads % 2 == 0 && groups > 1 && groups % 2 != 0 ? 1 : 0; // (pairs of KV heads: see the kernel)
 #define EARLY a.seq_lens, a.cu_seqlens_q, static_cast<int32_t>(a.index_type), a.num_seqs, a.capacity, a.runs
     if constexpr (!RUNS) {
