@@ -120,6 +120,10 @@ infiniStatus_t Descriptor::create(infiniopHandle_t handle, Descriptor **desc_ptr
     CHECK_RESULT(info);
     const PagedAttentionPrefillFp4Info in = info.take();
     const int units = device::amd::deviceInfo(handle->device_id).compute_units;
+    if (workgroups(static_cast<int64_t>(in.num_rows * in.num_heads / in.pool.num_kv_heads), static_cast<int64_t>(in.num_seqs),
+                   static_cast<int64_t>(in.pool.num_kv_heads), 64) >= 0x1000000) { // (2^32 threads)
+        return INFINI_STATUS_BAD_TENSOR_SHAPE;
+    }
     Opaque o{};
     o.wide = wideBlocks(in, units);
     o.by_length = byLength(in, units);

@@ -45,10 +45,11 @@ def sequence(codes, scales, pages, tokens):
     return x.transpose(0, 1).flatten(1, 2)[:, :tokens]
 
 
-def attention(q, k, v, scale, last, slopes=None):
+def attention(q, k, v, scale, last, slopes=None, terms=False):
     """q [n, heads, d] over k, v [KV heads, tokens, d]: row j sees tokens 0 .. last[j] (none where last[j] < 0: the row is
     NaN, to be left out by the caller). A token that a row does not see has no part in it, whatever it holds.
-    Returns the outputs, and how far a kernel of the kind tested may be off before it rounds them (`allowed`)."""
+    Returns the outputs, and how far a kernel of the kind tested may be off before it rounds them (`allowed`); `terms`: one
+    that takes the query as three 6-bit terms."""
     n, heads, d = q.shape
     tokens = k.shape[1]
     group = heads // k.shape[0]
@@ -68,20 +69,28 @@ def attention(q, k, v, scale, last, slopes=None):
         o = p @ torch.where(finite, vh, 0.0)
         o = o + torch.where(sees.double() @ (~finite).double() > 0, math.nan, 0.0)  # a value that a row sees and is not finite
         out[rows, h] = o[rows]
-        allowed[rows, h] = _allowed(x[:, h], kh, vh, s, p, scale, sees)[rows]
+        allowed[rows, h] = _allowed(x[:, h], kh, vh, s, p, scale, sees, terms)[rows]
     return out, allowed
 
 
-def _allowed(x, k, v, s, p, scale, sees):
+def _allowed(x, k, v, s, p, scale, sees, terms):
     """Before the outputs are rounded. Scores are fp32 sums of d exact products of up to sum |q| |k|, each addition rounded
     (2^-24), the sum times the scale, a bias and log2(e) (four more roundings of the score's size); exp2 is good to 2^-22 of its
     value. An error of e in a score is one of e in a probability's logarithm. Probabilities go to the matrix unit in fp16: 2^-11
     of their value, and below 2^-14 half a step of 2^-24, against a largest one of at least 1; the denominator sums them in
-    fp32 unrounded (tokens additions, in at most 64 lanes and partial results: 2^-24 each over tokens / 16)."""
+    fp32 unrounded (tokens additions, in at most 64 lanes and partial results: 2^-24 each over tokens / 16).
+    `terms`: 32 elements of the query are the sum of three rows of e2m3 (steps of 1/8 below 2, of 1/4 below 4) under scales s,
+    2^-5 s, 2^-10 s, s the power of two with max / s in [2, 4). The first rounding leaves at most s / 8 = 4 (2^-5 s), the second
+    at most 2^-5 s / 8 = 4 (2^-10 s), the third 2^-10 s / 8 <= 2^-14 max: that much of every element's |k| in the score."""
     d, tokens = k.shape[-1], k.shape[0]
     magnitude = (x.abs() @ torch.nan_to_num(k).abs().T * abs(scale)).masked_fill(~sees, 0.0).amax(-1)
     score = torch.where(sees, torch.nan_to_num(s.abs(), posinf=0.0), 0.0).amax(-1)
-    e = magnitude * (d + 2) * 2.0 ** -24 + score * 4 * 2.0 ** -24 + 2.0 ** -22
+    rounded = 0.0
+    if terms:
+        top = x.abs().unflatten(-1, (d // GROUP, GROUP)).amax(-1)
+        weight = torch.nan_to_num(k).abs().unflatten(-1, (d // GROUP, GROUP)).sum(-1)
+        rounded = (top @ weight.T * abs(scale)).masked_fill(~sees, 0.0).amax(-1) * 2.0 ** -14
+    e = rounded + magnitude * (d + 2) * 2.0 ** -24 + score * 4 * 2.0 ** -24 + 2.0 ** -22
     relative = 2 * e + 2.0 ** -11 + (tokens / 16 + 16) * 2.0 ** -24
     w = torch.nan_to_num(v).abs()
     return torch.nan_to_num(p) @ w * relative[:, None] + (sees.double() @ w) * 2.0 ** -25
@@ -103,6 +112,13 @@ def make_pool(seed, blocks, heads, page, size, *, spread=1.0):
         channel = torch.exp(spread * torch.randn((heads, 1, size), generator=gen))
         made.append(quantise(torch.randn((blocks, heads, page, size), generator=gen) * channel))
     return made[0][0], made[1][0], made[0][1], made[1][1]
+
+
+def widen(b, entries):
+    """The batch with a block table that is `entries` wider than it needs, of pages that do not exist."""
+    table = b["table"]
+    more = torch.full((table.shape[0], entries), 1 << 30, dtype=torch.int64, device=table.device)
+    return dict(b, table=torch.cat((table, more.to(table.dtype)), 1))
 
 
 def make_batch(seed, lens, heads, kv_heads, d, page, dtype, *, index=torch.int64, layout="packed", spare=3, poison=True, hot=None, rows=None):

@@ -60,6 +60,41 @@ def test_lengths_sizes_pages(dtype, d, page):
     check(fp4.make_batch(d + page, BORDERS, 8, 2, d, page, dtype), BORDERS)
 
 
+# A table that could hold far more tokens than the sequences have: their steps are cut into equal runs.
+WIDE = 1 << 16
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("page", [16, 32, 8, 24, 1, 7, 48])
+def test_cut_lengths_sizes_pages(dtype, d, page):
+    print("case", dtype, d, page, flush=True)
+    check(fp4.widen(fp4.make_batch(d + page, BORDERS, 8, 2, d, page, dtype), WIDE), BORDERS)
+
+
+@pytest.mark.parametrize("sequences", [1, 3, 65, 200])
+@pytest.mark.parametrize("heads,kv_heads", [(8, 2), (40, 1), (3, 3), (34, 2)])
+def test_cut_parts_of_a_row(sequences, heads, kv_heads):
+    """Joined by one wavefront, by four and by sixteen; more sequences than lanes; pairs of KV heads and single ones."""
+    lens = [(137 * i) % 400 + (3000 if i == 0 else 0) for i in range(sequences)]
+    slopes = torch.tensor([2.0 ** (-h / 4) for h in range(heads)], device=DEV)
+    for index in (torch.int64, torch.int32, torch.uint32):
+        b = fp4.widen(fp4.make_batch(21, lens, heads, kv_heads, 128, 16, torch.bfloat16, index=index, layout="padded"), WIDE)
+        check(b, lens)
+        check(b, lens, slopes)
+
+
+def test_cut_and_whole_agree_on_a_nan():
+    lens = [70, 1000, 129]
+    b = fp4.widen(fp4.make_batch(11, lens, 8, 2, 128, 16, torch.bfloat16), WIDE)
+    clean = check(b, lens)
+    b["pool"][3][int(b["table"][1, 17]), 1, 5, 2] = NAN_BYTE
+    got = ops.paged_attention_fp4(b["q"], *b["pool"], b["table"], b["lens"], None, b["scale"])
+    nan = torch.zeros_like(got, dtype=torch.bool)
+    nan[1, 4:, 64:96] = True
+    assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], clean[~nan])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("heads,kv_heads", [(1, 1), (8, 8), (32, 8), (40, 8), (28, 4), (48, 8), (16, 1), (17, 1), (64, 2), (40, 1), (3, 3)])
 def test_head_layouts(dtype, heads, kv_heads):

@@ -41,7 +41,7 @@ def reference(b, slopes=None):
         pages = b["table"][i, :b["needed"][i]].long()
         k, v = fp4.sequence(pool[0], pool[2], pages, n + h), fp4.sequence(pool[1], pool[3], pages, n + h)
         last = [h + j for j in range(n)]
-        out[at], allowed[at] = fp4.attention(q[at], k, v, b["scale"], last, slopes)
+        out[at], allowed[at] = fp4.attention(q[at], k, v, b["scale"], last, slopes, terms=True)
         rows[at] = torch.tensor([x >= 0 for x in last], device=DEV)
     return out, allowed, rows
 
@@ -70,6 +70,100 @@ RUNS = [(1, 0), (0, 5), (2, 0), (17, 0), (64, 0), (5, 59), (3, 61), (1, 300), (6
 def test_runs_sizes_pages(dtype, d, page):
     print("case", dtype, d, page, flush=True)
     check(make_runs(d + page, RUNS, 8, 2, d, page, dtype, lead=3, behind=5))
+
+
+# A table that could hold far more tokens than the sequences have: their few rows go to the wavefronts of the whole device, 16 at
+# a time, whatever the lengths are.
+WIDE = 1 << 16
+FEW = [(1, 0), (2, 0), (0, 7), (5, 59), (3, 61), (1, 300), (4, 28), (0, 0), (4, 640), (3, 509), (4, -2), (3, -3), (9, 33)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("page", [16, 32, 8, 24, 1, 7, 48])
+def test_few_rows_sizes_pages(dtype, d, page):
+    print("case", dtype, d, page, flush=True)
+    check(fp4.widen(make_runs(d + page, FEW, 8, 2, d, page, dtype, lead=3, behind=5), WIDE))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (8, 8), (32, 8), (40, 8), (28, 4), (48, 8), (16, 1), (17, 1), (64, 2), (3, 3)])
+def test_few_rows_head_layouts(dtype, heads, kv_heads):
+    check(fp4.widen(make_runs(heads, [(3, 700), (1, 40), (4, 0), (2, 333)], heads, kv_heads, 128, 16, dtype), WIDE))
+
+
+@pytest.mark.parametrize("sequences", [1, 3, 65, 200])
+def test_few_rows_parts_of_a_row(sequences):
+    """Joined by one wavefront, by four and by sixteen; more sequences than lanes."""
+    runs = [(1 + i % 4, (137 * i) % 400 + (3000 if i == 0 else 0)) for i in range(sequences)]
+    slopes = torch.tensor([2.0 ** -h for h in range(8)], device=DEV)
+    for index in (torch.int64, torch.int32, torch.uint32):
+        b = fp4.widen(make_runs(21, runs, 8, 2, 64, 16, torch.float16, index=index, layout="rows"), WIDE)
+        check(b)
+        check(b, slopes)
+        check(dict(b, scale=-0.1))
+
+
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("page", [16, 8, 7])
+def test_few_rows_and_values_that_are_not_finite(d, page):
+    runs = [(4, 190), (5, 66), (7, 28), (1, 5)]
+    b = fp4.widen(make_runs(11, runs, 8, 2, d, page, torch.bfloat16), WIDE)
+    for i, (n, h) in enumerate(runs):
+        for pool, back, group in ((2, 1, 0), (3, 2, 1), (3, n - 1, d // 32 - 1)):
+            t = h + max(n - back, 0)
+            if t < h + n:
+                b["pool"][pool][int(b["table"][i, t // page]), 1, t % page, group] = fp4.NAN_BYTE
+    got = check(b)
+    assert got.isnan().any() and not got[:, :4].isnan().any()
+
+
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_values_that_are_not_finite_in_the_history(d, slopes):
+    """Keys and values in steps that every row of a block sees to the end: they reach all of them, in their columns."""
+    runs = [(90, 300), (40, 129), (66, 64)]
+    slopes = torch.tensor([2.0 ** -h for h in range(8)], device=DEV) if slopes else None
+    b = make_runs(12, runs, 8, 2, d, 16, torch.bfloat16)
+    for i, pool, t in ((0, 3, 0), (0, 3, 63), (0, 3, 200), (0, 3, 299), (1, 3, 127), (2, 2, 10)):
+        b["pool"][pool][int(b["table"][i, t // 16]), 1, t % 16, t % (d // 32)] = fp4.NAN_BYTE
+    got = check(b, slopes)
+    assert not got[:, :4].isnan().any() and got[130:, 4:].isnan().all() and not got[:130, 4:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 192, 256])
+def test_queries_of_every_size(dtype, d):
+    """Elements of one group from the type's largest to its smallest, groups of zeros, and queries that are not finite."""
+    runs = [(40, 30)]
+    b = make_runs(13, runs, 8, 2, d, 16, dtype)
+    gen = torch.Generator().manual_seed(5)
+    q = torch.randn(b["q"].shape, generator=gen).double()
+    q[:20] *= torch.exp2(torch.randint(-16, 3, q[:20].shape, generator=gen).double())
+    q[3] = 0
+    q[4, :, 32:] = 0
+    q[5] *= 2.0 ** -20
+    b["q"] = q.to(dtype).to(DEV)
+    check(b)
+    big = 300.0
+    b["q"] = (q * big).to(dtype).to(DEV)
+    check(b)
+    clean = check(b)
+    b["q"] = b["q"].clone()
+    b["q"][7, 1, d - 1] = math.inf
+    b["q"][8, 2, 0] = math.nan
+    got = ops.paged_attention_prefill_fp4(b["q"], *b["pool"], b["table"], b["lens"], b["cum"], None, b["scale"])
+    nan = torch.zeros_like(got, dtype=torch.bool)
+    nan[7, 1] = nan[8, 2] = True
+    assert torch.equal(got.isnan(), nan) and torch.equal(got[~nan], clean[~nan])
+
+
+def test_blocks_in_both_orders():
+    """More row blocks than compute units: by length up to 64 sequences, as the sequences come beyond."""
+    runs = [((53 * i) % 90, (37 * i) % 130) for i in range(64)]
+    check(make_runs(31, runs, 32, 8, 64, 16, torch.bfloat16))
+    check(make_runs(32, runs + [(5, 0), (40, 3)], 32, 8, 64, 16, torch.bfloat16))
+    check(make_runs(33, [(1, -5), (600, -590), (700, 0), (3, -1), (300, 40)], 16, 4, 64, 16, torch.float16))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
@@ -177,7 +271,7 @@ def test_page_order_repeats_and_lengths_beyond_the_table():
     want = torch.full_like(b["q"], 7.0, dtype=torch.float64)
     pages = b["table"][0].long()
     k, v = (fp4.sequence(b["pool"][x], b["pool"][x + 2], pages, 160) for x in (0, 1))
-    want, allowed = fp4.attention(b["q"], k, v, b["scale"], [159] * 100)
+    want, allowed = fp4.attention(b["q"], k, v, b["scale"], [159] * 100, terms=True)
     got = ops.paged_attention_prefill_fp4(b["q"], *b["pool"], b["table"], b["lens"], b["cum"], None, b["scale"])
     assert fp4.off_by(got, want, allowed) <= 1.0
     # prefix sums beyond the query: clipped
@@ -268,16 +362,17 @@ def test_chunks_through_the_whole_family():
         rows = torch.arange(20, device=DEV).view(1, 20)
         wide = ops.paged_attention_prefill(q, *as_pool, rows, lens, cum, None, d ** -0.5)
         exact, allowed = fp4.attention(q, ko[:total].transpose(0, 1).double(), vo[:total].transpose(0, 1).double(), d ** -0.5,
-                                       list(range(total - n, total)))
+                                       list(range(total - n, total)), terms=n > 1)
         assert fp4.off_by(got, exact, allowed) <= 1.0
         # the 16-bit operator rounds its probabilities to bf16: 2^-8 of every weight, twice (numerator and denominator)
         assert fp4.off_by(wide, exact, allowed + 2 ** -7 * vo[:total].abs().amax().double()) <= 1.0
         assert torch.equal(ko[:total].cpu().double()[-n:], fp4.values(*fp4.quantise(k.cpu())))
 
 
-def test_c_entry_points():
-    runs = [(70, 30), (2, 500)]
-    b = make_runs(15, runs, 16, 4, 128, 16, torch.bfloat16)
+@pytest.mark.parametrize("wide", [0, WIDE])
+def test_c_entry_points(wide):
+    runs = [(7, 30), (2, 500)] if wide else [(70, 30), (2, 500)]
+    b = fp4.widen(make_runs(15, runs, 16, 4, 128, 16, torch.bfloat16), wide)
     out = torch.full_like(b["q"], 7.0)
     tensors = [out, b["q"], *b["pool"], b["table"], b["lens"], b["cum"]]
     L.set_device(L.InfiniDevice.AMD, 0)
@@ -303,6 +398,7 @@ def test_c_entry_points():
             torch.cuda.synchronize()
             assert fp4.off_by(out, want, allowed) <= 1.0
     S = L.InfiniStatus
+    assert (size.value > 0) == (wide > 0)
     if size.value:
         assert run(ptr(workspace), size.value - 1, *pointers) == S.INSUFFICIENT_WORKSPACE
         assert run(None, size.value, *pointers) == S.INSUFFICIENT_WORKSPACE
