@@ -6,7 +6,7 @@
 // piece of LDS (global_load_lds, no register in between), several steps ahead: a step is 4.4 KB at head 128, and at the rate
 // of the memory some 25 KB per compute unit have to be in flight for every microsecond that a load takes. (Held in registers
 // instead, 26 of them a step, one step ahead was all there was room for: 128 sequences of 1 024 - 8 192, 64 / 8 heads of 128,
-// 151 us, 4.3 TB/s.) lane = 16 g + c (g = 0..3, c = 0..15). Per tile:
+// 151 us, 4.3 TB/s; now 128 us, 5.0 TB/s, and 113 us with the arithmetic left out.) lane = 16 g + c (g = 0..3, c = 0..15). Per tile:
 //   S[token][head] = K . Q^T   v_mfma_f32_16x16x32, A = K: lane c holds HEAD / 4 neighbouring elements of one token. The
 //                              matrix instruction sums over the elements whatever their order, as long as the query has the
 //                              same, so a lane's elements need not be spread over the four groups g, and each lane's codes

@@ -31,12 +31,12 @@ inline int groupsPerUnit(size_t head) {
 // Whether every sequence is left to one workgroup per KV head (and 16 query heads): no scan of the lengths in front, no partial
 // results and no second kernel, but as long as the longest sequence, and whole rounds of workgroups. `steps`: of the longest
 // that the table can hold. us cut into runs / whole, bf16, lengths between half of and the given tokens:
-//   head 128, 64 / 8 heads: 500 tokens 64 workgroups 10.3 / 7.2, 256 18.3 / 7.9, 512 22.0 / 14.7, 1 024 27.7 / 27.1; 1 000 tokens 8
-//   9.1 / 8.0, 256 22.2 / 11.1, 512 26.7 / 21.3, 1 024 36.5 / 39.9; 2 000 tokens 8 10.3 / 11.0, 64 16.7 / 13.7, 256 26.4 / 16.5, 512
-//   35.3 / 30.6, 1 024 53.8 / 57.4; 4 000 tokens 64 21.1 / 22.8, 200 30.6 / 24.8, 256 35.3 / 26.0 (300 - 4 000 30.2 / 24.6), 400 43.7 /
-//   43.9 (37.2 / 38.8); 32 / 8 heads, 4 096 - 8 192 256 49.2 / 46.4, 500 - 8 192 39.1 / 42.9.
-//   head 64 (two such workgroups to a compute unit): 4 000 tokens 128 16.2 / 18.9, 192 19.8 / 20.3, 512 32.8 / 29.7; head 192: 1 000
-//   tokens 8 10.2 / 10.6, 2 000 64 18.2 / 18.6, 400 38.5 / 38.9; head 256: 1 000 tokens 8 10.8 / 11.9, 64 16.4 / 13.7.
+//   head 128, 64 / 8 heads: 500 tokens 64 workgroups 12.3 / 7.3, 256 14.7 / 8.0, 512 20.9 / 14.7, 1 024 29.8 / 27.0; 1 000 tokens 8
+//   8.7 / 8.1, 256 19.2 / 11.2, 512 27.1 / 21.2, 1 024 39.6 / 40.1; 2 000 tokens 8 9.1 / 10.8, 64 14.7 / 13.5, 256 23.1 / 16.1, 512
+//   33.5 / 30.4, 1 024 57.2 / 57.2; 4 000 tokens 64 18.0 / 22.9, 200 28.3 / 24.9, 256 31.7 / 25.6 (300 - 4 000 29.7 / 24.6), 400 41.9 /
+//   44.9 (36.7 / 38.8).
+//   head 64 (two such workgroups to a compute unit): 4 000 tokens 128 16.5 / 18.9, 192 20.1 / 20.2, 512 33.8 / 29.9; head 192: 1 000
+//   tokens 8 10.6 / 10.4, 2 000 64 17.2 / 18.6, 512 41.9 / 41.0; head 256: 1 000 tokens 8 11.0 / 12.3, 64 16.1 / 14.1.
 inline bool wholeSequences(int64_t workgroups, int64_t steps, size_t head, int compute_units) {
     const int64_t slots = static_cast<int64_t>(compute_units) * (head == 64 ? Layout<64>::kWholePerUnit : Layout<128>::kWholePerUnit);
     if (steps <= 32) {

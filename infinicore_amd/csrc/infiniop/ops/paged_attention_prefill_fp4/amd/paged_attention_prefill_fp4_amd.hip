@@ -83,18 +83,18 @@ bool byLength(const PagedAttentionPrefillFp4Info &in, int units) {
     return in.num_seqs <= 64 && static_cast<int64_t>(in.num_rows * in.num_heads) / 64 > units;
 }
 
-// Whether rows of 16, whose tokens the wavefronts of the whole chip divide among themselves (decode_fp4.h), beat row blocks
+// Whether rows of 16, whose tokens the workgroups of the whole chip divide among themselves (decode_fp4.h), beat row blocks
 // of 64 that each walk all of theirs. A row block takes 0.9 us per 64 tokens on its own and 0.6 us of a compute unit's time;
-// 16 rows take 0.36 us of it, and dividing and joining 12 us. (Head 128; how much a table holds stands for the lengths.)
-// Measured, row blocks / rows of 16, in us: 32 sequences of 6000 tokens, 8 KV heads: 8 rows each 89 / 55, 32 rows 90 / 86 - 97,
-// 64 rows 92 / 145; of 1000 tokens: 8 rows 23 / 22, 32 rows 24 / 33; 1 sequence of 20000: 128 rows 270 / 45; head 64: 32 of 6000, 8
-// rows 80 / 42, 64 rows 82 / 109; head 256: 142 / 94, 147 / 235.
+// 16 rows take 0.38 us of it, and dividing and joining 8 us. (Head 128; how much a table holds stands for the lengths.)
+// Measured, row blocks / rows of 16, in us: 32 sequences of 6000 tokens, 8 KV heads: 8 rows each 87 / 45, 32 rows 88 / 79,
+// 64 rows 89 / 154; of 1000 tokens: 8 rows 21 / 18, 32 rows 22 / 24; 8 of 1000: 64 rows 21 / 19, 128 23 / 23; 1 sequence of 20000:
+// 128 rows 268 / 41; head 64: 32 of 6000, 32 rows 79 / 62, 64 rows 80 / 107; head 256: 140 / 140, 144 / 268.
 bool fewRows(const PagedAttentionPrefillFp4Info &in, int units) {
     const double steps = (0.6 + 0.4 / 128 * static_cast<double>(in.head_size)) * std::max(1.0, static_cast<double>(in.capacity()) / 64);
     const double seqs = static_cast<double>(in.num_seqs), rows = static_cast<double>(in.num_rows * in.num_heads / in.pool.num_kv_heads);
     const double heads_per_unit = static_cast<double>(in.pool.num_kv_heads) / units;
     const double blocks = seqs * std::ceil(rows / seqs / 64) * heads_per_unit, chunks = seqs * std::ceil(rows / seqs / 16) * heads_per_unit;
-    return 12 + 0.36 * steps * chunks < steps * std::max(0.9, 0.6 * blocks);
+    return 8 + 0.38 * steps * chunks < steps * std::max(0.9, 0.6 * blocks);
 }
 
 } // namespace
