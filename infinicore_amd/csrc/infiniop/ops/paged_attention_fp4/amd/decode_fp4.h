@@ -885,11 +885,23 @@ decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_ty
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     auto work = [&](int seq) { return workOf<RUNS>(index_type, seq_lens, cu_seqlens_q, capacity, RUNS ? a.total_q_tokens : 0, RUNS ? a.group : 0, seq); };
 
+    // The work of 64 sequences, one a lane. RUNS: rows that several sequences claim (prefix sums that fall) are more than the
+    // query has, and the partial results have room for that many: sequences beyond have none.
+    int rows_before = 0;
+    auto worksFrom = [&](int base) {
+        Work w = base + lane < num_seqs ? work(base + lane) : Work{};
+        if constexpr (RUNS) {
+            const int sum = rows_before + waveInclusiveSum(w.q_len);
+            w = sum > a.total_q_tokens ? Work{} : w;
+            rows_before = min(__builtin_amdgcn_readlane(sum, 63), a.total_q_tokens + 1);
+        }
+        return w;
+    };
     // all steps, and with up to 64 sequences the work of each in a lane
     Work mine{};
     uint32_t total = 0, segments_of_all = 0;
     for (int base = 0; base < num_seqs; base += 64) {
-        mine = base + lane < num_seqs ? work(base + lane) : Work{};
+        mine = worksFrom(base);
         total += __builtin_amdgcn_readlane(waveInclusiveSum(static_cast<unsigned>(mine.all())), 63);
         if constexpr (RUNS) {
             segments_of_all += __builtin_amdgcn_readlane(waveInclusiveSum(mine.steps > 0 ? mine.segments : 0), 63);
@@ -915,9 +927,10 @@ decodeFp4Kernel(const void *seq_lens, const void *cu_seqlens_q, int32_t index_ty
     Rows rows(a);
 
     uint32_t before = 0, segments_before = 0; // of the sequences in front of the 64 at hand
+    rows_before = 0;
     for (int base = 0; base < num_seqs && at < end; base += 64) {
         if (num_seqs > 64) {
-            mine = base + lane < num_seqs ? work(base + lane) : Work{};
+            mine = worksFrom(base);
         }
         const uint32_t sum = waveInclusiveSum(static_cast<unsigned>(mine.all()));
         const uint32_t segment_sum = RUNS ? waveInclusiveSum(static_cast<unsigned>(mine.steps > 0 ? mine.segments : 0)) : 0;

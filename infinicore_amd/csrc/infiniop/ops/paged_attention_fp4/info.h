@@ -104,6 +104,7 @@ struct AttentionFp4Info {
         const fp4::PoolInfo &p = info.pool;
         for (ptrdiff_t row : {p.k_codes.row, p.v_codes.row, p.k_scales.row, p.v_scales.row}) {
             CHECK_OR_RETURN(row >= 0 && row <= 0xffffff, INFINI_STATUS_BAD_TENSOR_STRIDES);
+            CHECK_OR_RETURN(p.block_size <= 0x7fffffff / static_cast<size_t>(row > 0 ? row : 1), INFINI_STATUS_BAD_TENSOR_STRIDES);
         }
         // outputs of two rows or heads at one place would be written by different wavefronts
         CHECK_OR_RETURN((out_desc->dim(0) <= 1 || out_desc->stride(0) != 0) && (out_desc->dim(1) <= 1 || out_desc->stride(1) != 0),

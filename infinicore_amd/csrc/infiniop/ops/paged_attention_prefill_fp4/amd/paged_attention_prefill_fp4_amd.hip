@@ -127,7 +127,7 @@ infiniStatus_t Descriptor::create(infiniopHandle_t handle, Descriptor **desc_ptr
     Opaque o{};
     o.wide = wideBlocks(in, units);
     o.by_length = byLength(in, units);
-    if (fewRows(in, units)) {
+    if (in.num_rows < 0x1000000 && fewRows(in, units)) { // (the kernel sums 64 sequences' rows in 32 bits)
         o.plan = planDecode(in, true, units);
         o.few = o.plan.possible && static_cast<int64_t>(o.plan.max_segments) * o.plan.part_rows < 0x400000; // (2^32 threads of the merge)
     }

@@ -42,6 +42,11 @@ struct PagedCachingFp4Info {
             || k_desc->dim(2) != info.pool.k_size || v_desc->dim(2) != info.pool.v_size) {
             return INFINI_STATUS_BAD_TENSOR_SHAPE;
         }
+        // counted in 32 bits, 65 535 workgroups of 256 lanes of eight elements to a token
+        if (info.num_tokens > 0x3fffffff || info.pool.num_kv_heads > 0x7fff800 || info.pool.k_size + info.pool.v_size > 0x7fff800
+            || info.pool.num_kv_heads * (info.pool.k_size + info.pool.v_size) > 0x7fff800) {
+            return INFINI_STATUS_BAD_TENSOR_SHAPE;
+        }
         CHECK_OR_RETURN(k_desc->stride(2) == 1 || k_desc->dim(2) == 0, INFINI_STATUS_BAD_TENSOR_STRIDES);
         CHECK_OR_RETURN(v_desc->stride(2) == 1 || v_desc->dim(2) == 0, INFINI_STATUS_BAD_TENSOR_STRIDES);
         CHECK_OR_RETURN(slot_mapping_desc->stride(0) == 1 || info.num_tokens <= 1, INFINI_STATUS_BAD_TENSOR_STRIDES);

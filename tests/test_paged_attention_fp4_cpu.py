@@ -75,6 +75,10 @@ def test_descriptors_refuse(lib, host_amd_handle, which):
         # rows that do not all begin where 16 bytes of codes, or four scales, are loaded at once
         odd = torch.zeros((*o[name].shape[:3], o[name].shape[3] + (8 if "codes" in name else 2)), dtype=torch.uint8)
         assert status(**{name: odd[..., :o[name].shape[3]]}) == S.BAD_TENSOR_STRIDES
+        # a page of more than 2^31 bytes
+        far = torch.empty_strided((6, 2, 1 << 12, o[name].shape[3]), (1 << 40, 1 << 38, 1 << 20, 1), dtype=torch.uint8, device="meta")
+        pages = {n: torch.empty((6, 2, 1 << 12, o[n].shape[3]), dtype=torch.uint8, device="meta") for n in _POOL}
+        assert status(**pages) == 0 and status(**{**pages, name: far}) == S.BAD_TENSOR_STRIDES
     assert status(q=o["q"].float(), out=o["out"].float()) == S.BAD_TENSOR_DTYPE
     assert status(out=o["out"].half()) == S.BAD_TENSOR_DTYPE
     for name in ("q", "out"):
@@ -104,6 +108,14 @@ def test_descriptors_refuse(lib, host_amd_handle, which):
         assert status(cum=o["cum"][:, None]) == S.BAD_TENSOR_SHAPE
         assert status(cum=o["cum"][:-1]) == S.BAD_PARAM
         assert status(cum=torch.zeros(8, dtype=torch.int64)[::2]) == S.BAD_TENSOR_STRIDES
+        for rows, expected in ((1 << 24, 0), (1 << 28, S.BAD_TENSOR_SHAPE)):  # more rows than are counted
+            q = torch.empty((rows, 8, 128), dtype=bf16, device="meta")
+            assert status(q=q, out=q) == expected
+        n = 65000  # more workgroups than a grid has
+        heads = torch.empty((n, 260, 128), dtype=bf16, device="meta")
+        pool = {name: torch.empty((6, 260, 16, o[name].shape[3]), dtype=torch.uint8, device="meta") for name in _POOL}
+        rest = {name: torch.empty(size, dtype=torch.int64, device="meta") for name, size in (("table", (n, 4)), ("lens", n), ("cum", n + 1))}
+        assert status(q=heads, out=heads, **pool, **rest) == S.BAD_TENSOR_SHAPE
     cpu = ctypes.pointer(lib.Handle(lib.InfiniDevice.CPU, 0))
     assert _create(lib, cpu, which, o) == S.DEVICE_TYPE_NOT_SUPPORTED
     assert _create(lib, None, which, o) == S.NULL_POINTER

@@ -370,6 +370,39 @@ def test_chunks_through_the_whole_family():
 
 
 @pytest.mark.parametrize("wide", [0, WIDE])
+def test_prefix_sums_that_fall(wide):
+    """Rows claimed by several sequences, all of them alike: written once or more, with what one of them gives them; nothing
+    outside q, the output and the workspace is reached (the workspace has a border that has to stay)."""
+    b = make_runs(41, [(4, 60)] * 70, 8, 2, 128, 16, torch.bfloat16, poison=False)
+    b["table"][:] = b["table"][:1].clone()
+    b = fp4.widen(b, wide)
+    b["q"] = b["q"][:8].contiguous()
+    b["q"][4:] = b["q"][:4].clone()
+    cum = torch.tensor([(0, 4, 8)[i % 3] for i in range(71)], device=DEV)
+    want, allowed, _ = reference(dict(b, runs=b["runs"][:2], starts=[0, 4, 8]))
+    L.set_device(L.InfiniDevice.AMD, 0)
+    handle = L.create_handle()
+    out = torch.zeros_like(b["q"])
+    tensors = [out, b["q"], *b["pool"], b["table"], b["lens"], cum]
+    descs = [describe(t) for t in tensors]
+    op, size = L.infiniopOperatorDescriptor_t(), ctypes.c_size_t(0)
+    L.check_error(L.LIBINFINIOP.infiniopCreatePagedAttentionPrefillFp4Descriptor(handle, ctypes.byref(op), *descs,
+                                                                                 L.infiniopTensorDescriptor_t(), b["scale"]))
+    L.check_error(L.LIBINFINIOP.infiniopGetPagedAttentionPrefillFp4WorkspaceSize(op, ctypes.byref(size)))
+    assert (size.value > 0) == (wide > 0)
+    workspace = torch.full((size.value + 4096,), 77, dtype=torch.uint8, device=DEV)
+    torch.cuda.synchronize()
+    L.check_error(L.LIBINFINIOP.infiniopPagedAttentionPrefillFp4(op, ptr(workspace), size.value, *(ptr(t) for t in tensors), None, None))
+    torch.cuda.synchronize()
+    assert (workspace[size.value:] == 77).all()
+    assert fp4.off_by(out, want, allowed) <= 1.0
+    for d in descs:
+        L.destroy_tensor_descriptor(d)
+    L.check_error(L.LIBINFINIOP.infiniopDestroyPagedAttentionPrefillFp4Descriptor(op))
+    L.destroy_handle(handle)
+
+
+@pytest.mark.parametrize("wide", [0, WIDE])
 def test_c_entry_points(wide):
     runs = [(7, 30), (2, 500)] if wide else [(70, 30), (2, 500)]
     b = fp4.widen(make_runs(15, runs, 16, 4, 128, 16, torch.bfloat16), wide)

@@ -124,6 +124,11 @@ def test_descriptors_refuse(lib, host_amd_handle, which):
     assert status(slots=o["slots"].int()) == S.BAD_TENSOR_DTYPE
     assert status(slots=o["slots"][:-1]) == S.BAD_TENSOR_SHAPE
     assert status(slots=torch.zeros(10, dtype=torch.int64)[::2]) == S.BAD_TENSOR_STRIDES
+    tokens = 1 << 30  # counted in 32 bits
+    many = {name: torch.empty((tokens, *o[name].shape[1:]), dtype=o[name].dtype, device="meta") for name in ("k", "v", "slots")}
+    assert status(**many) == S.BAD_TENSOR_SHAPE
+    wide = {name: torch.empty((*o[name].shape[:-1], o[name].shape[-1] << 22), dtype=o[name].dtype, device="meta") for name in (*_POOL, "k", "v")}
+    assert status(**wide) == S.BAD_TENSOR_SHAPE
     cpu = ctypes.pointer(lib.Handle(lib.InfiniDevice.CPU, 0))
     assert _create(lib, cpu, which, o) == S.DEVICE_TYPE_NOT_SUPPORTED
     assert _create(lib, None, which, o) == S.NULL_POINTER
