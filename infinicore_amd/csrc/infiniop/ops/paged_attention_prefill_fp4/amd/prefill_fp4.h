@@ -245,61 +245,66 @@ __global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args
     int visible[R];
     float slope[R];
     int most_visible = 0, least_visible = 0x7fffffff;
+    auto takeQueries = [&]() {
+        uint4 x[R][G::kSets][4]; // all loads in front of the first use
+        bool valid[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int row = block_row0 + (w * R + r) * 16 + c;
-        const bool valid = row < total_rows;
-        const int token = valid ? row / a.group : 0;
-        const int head = kv_head * a.group + (valid ? row - token * a.group : 0);
-        visible[r] = valid ? visibleTokens(a, span, token) : 0;
-        slope[r] = a.alibi_slopes != nullptr && valid ? a.alibi_slopes[head] * kLog2e : 0.0f;
-        const S *from = static_cast<const S *>(a.q) + (span.q_start + token) * a.q_stride + head * a.q_head_stride;
+        for (int r = 0; r < R; ++r) {
+            const int row = block_row0 + (w * R + r) * 16 + c;
+            valid[r] = row < total_rows;
+            const int token = valid[r] ? row / a.group : 0;
+            const int head = kv_head * a.group + (valid[r] ? row - token * a.group : 0);
+            visible[r] = valid[r] ? visibleTokens(a, span, token) : 0;
+            slope[r] = a.alibi_slopes != nullptr && valid[r] ? a.alibi_slopes[head] * kLog2e : 0.0f;
+            const S *from = static_cast<const S *>(a.q) + (span.q_start + token) * a.q_stride + head * a.q_head_stride;
+            if (a.q_aligned) {
 #pragma unroll
-        for (int i = 0; i < (G::kProducts + 3) / 4; ++i) {
-            q_scales[r][i] = 0;
+                for (int i = 0; i < 4 * G::kSets; ++i) {
+                    x[r][i / 4][i % 4] = reinterpret_cast<const uint4 *>(from + 32 * G::chunkOf(i / 4, g))[i % 4];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4 * G::kSets; ++i) {
+                    const uint16_t *e = reinterpret_cast<const uint16_t *>(from + 32 * G::chunkOf(i / 4, g)) + 8 * (i % 4);
+                    x[r][i / 4][i % 4] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+                }
+            }
         }
 #pragma unroll
-        for (int set = 0; set < G::kSets; ++set) {
-            const S *at = from + 32 * G::chunkOf(set, g);
-            mx::f32x16 even, odd;
+        for (int r = 0; r < R; ++r) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t x[4];
-                if (a.q_aligned) {
-                    const uint4 y = reinterpret_cast<const uint4 *>(at)[i];
-                    x[0] = y.x, x[1] = y.y, x[2] = y.z, x[3] = y.w;
-                } else {
-                    const uint16_t *e = reinterpret_cast<const uint16_t *>(at) + 8 * i;
+            for (int i = 0; i < (G::kProducts + 3) / 4; ++i) {
+                q_scales[r][i] = 0;
+            }
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        x[j] = e[2 * j] | static_cast<uint32_t>(e[2 * j + 1]) << 16;
+            for (int set = 0; set < G::kSets; ++set) {
+                mx::f32x16 even, odd;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint4 y = x[r][set][i / 4];
+                    const uint32_t word = i % 4 == 0 ? y.x : i % 4 == 1 ? y.y : i % 4 == 2 ? y.z : y.w, pair = valid[r] ? word : 0u;
+                    even[i] = T::toFloat(__builtin_bit_cast(S, static_cast<uint16_t>(pair)));
+                    odd[i] = T::toFloat(__builtin_bit_cast(S, static_cast<uint16_t>(pair >> 16)));
+                }
+                const mx::Terms terms = mx::termsOf(even, odd);
+#pragma unroll
+                for (int m = set; m < G::kProducts; m += G::kSets) {
+                    const int term = G::termOf(m, g);
+                    mx::u32x6 codes;
+#pragma unroll
+                    for (int i = 0; i < 6; ++i) {
+                        codes[i] = term == 0 ? terms.codes[0][i] : term == 1 ? terms.codes[1][i] : term == 2 ? terms.codes[2][i] : 0u;
                     }
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t pair = valid ? x[j] : 0u;
-                    even[4 * i + j] = T::toFloat(__builtin_bit_cast(S, static_cast<uint16_t>(pair)));
-                    odd[4 * i + j] = T::toFloat(__builtin_bit_cast(S, static_cast<uint16_t>(pair >> 16)));
+                    q_codes[r][m] = codes;
+                    q_scales[r][m / 4] |= (term == 0 ? terms.scale[0] : term == 1 ? terms.scale[1] : terms.scale[2]) << (8 * (m % 4));
                 }
             }
-            const mx::Terms terms = mx::termsOf(even, odd);
-#pragma unroll
-            for (int m = set; m < G::kProducts; m += G::kSets) {
-                const int term = G::termOf(m, g);
-                mx::u32x6 codes;
-#pragma unroll
-                for (int i = 0; i < 6; ++i) {
-                    codes[i] = term == 0 ? terms.codes[0][i] : term == 1 ? terms.codes[1][i] : term == 2 ? terms.codes[2][i] : 0u;
-                }
-                q_codes[r][m] = codes;
-                q_scales[r][m / 4] |= (term == 0 ? terms.scale[0] : term == 1 ? terms.scale[1] : terms.scale[2]) << (8 * (m % 4));
-            }
+            most_visible = max(most_visible, visible[r]);
+            least_visible = min(least_visible, valid[r] ? visible[r] : 0x7fffffff);
         }
-        most_visible = max(most_visible, visible[r]);
-        least_visible = min(least_visible, valid ? visible[r] : 0x7fffffff);
-    }
-    most_visible = __builtin_amdgcn_readfirstlane(waveMaxInt(most_visible));
-    least_visible = __builtin_amdgcn_readfirstlane(-waveMaxInt(-least_visible));
+        most_visible = __builtin_amdgcn_readfirstlane(waveMaxInt(most_visible));
+        least_visible = __builtin_amdgcn_readfirstlane(-waveMaxInt(-least_visible));
+    };
 
     // ---- loads: codes and scales of this wavefront's tile of a step (WAVES = 8: of one pass over it) ----
     constexpr int kWavesPerTile = WAVES / kTiles;
@@ -329,6 +334,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args
     int t_next = kTile * own_tile;
     int batch = 0, ids = 0, ids_next = 0;
     int entry = 0, row_in_page = 0;
+    const int step_entries = BN / a.block_size, step_rows = BN - step_entries * a.block_size; // (WHOLE) from tile to tile
     auto lookUp = [&]() {
         const int token = min(t_next + (lane & 15), block_visible - 1);
         entry = token / a.block_size;
@@ -360,13 +366,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args
             const int e = inside ? entry : last_entry, row0 = inside ? row_in_page : (block_visible - 1) / kTile * kTile - last_entry * a.block_size;
             const int64_t id = __builtin_amdgcn_readlane(ids, e & 63);
             t_next += BN;
-            row_in_page += BN;
-#pragma unroll
-            for (int i = 0; i < BN / 16; ++i) { // (pages of 16 tokens or more)
-                const bool over = row_in_page >= a.block_size;
-                row_in_page -= over ? a.block_size : 0;
-                entry += over ? 1 : 0;
-            }
+            row_in_page += step_rows;
+            const int over = row_in_page >= a.block_size ? 1 : 0;
+            row_in_page -= over * a.block_size;
+            entry += step_entries + over;
             auto tile = [&](const PoolSide &s) { return s.base + id * s.block + kv_head * s.head + static_cast<int64_t>(row0) * s.row; };
             const char *k_codes = tile(a.k_codes), *k_scales = tile(a.k_scales);
 #pragma unroll
@@ -507,11 +510,12 @@ __global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args
                 }
             }
             if (!FULL && t0 + BN > least_visible) {
+                const int left = visible[r] - t0 - 4 * g; // of the lane's tokens 16 tt + i
 #pragma unroll
                 for (int tt = 0; tt < TT; ++tt) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        s[r][tt][i] = t0 + 16 * tt + 4 * g + i >= visible[r] ? -INFINITY : s[r][tt][i];
+                        s[r][tt][i] = 16 * tt + i >= left ? -INFINITY : s[r][tt][i];
                     }
                 }
             }
@@ -572,14 +576,22 @@ __global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args
             }
         }
         if (!FULL && step >= full_steps) {
+            unsigned long long noted[G::kGroups], any = 0;
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int n = visible[r] - t0;
-                const unsigned long long sees = n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1);
+            for (int i = 0; i < G::kGroups; ++i) {
+                noted[i] = bad[step - full_steps][i];
+                any |= noted[i];
+            }
+            if (__builtin_amdgcn_ballot_w64(any != 0) != 0) {
 #pragma unroll
-                for (int e = 0; e < G::kCols; ++e) {
-                    if ((bad[step - full_steps][e / 2] & sees) != 0) {
-                        o[r][e] = f32x4{NAN, NAN, NAN, NAN};
+                for (int r = 0; r < R; ++r) {
+                    const int n = visible[r] - t0;
+                    const unsigned long long sees = n <= 0 ? 0ull : (n >= 64 ? ~0ull : (1ull << n) - 1);
+#pragma unroll
+                    for (int e = 0; e < G::kCols; ++e) {
+                        if ((noted[e / 2] & sees) != 0) {
+                            o[r][e] = f32x4{NAN, NAN, NAN, NAN};
+                        }
                     }
                 }
             }
@@ -589,6 +601,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args
     // ---- pipeline: codes two steps ahead in registers, values one step ahead in LDS ----
     turnPages();
     load();
+    takeQueries(); // (while the first tile is on its way)
     __syncthreads(); // the notes of values that are not finite are clear
     convert(0, std::false_type{});
     turnPages();
