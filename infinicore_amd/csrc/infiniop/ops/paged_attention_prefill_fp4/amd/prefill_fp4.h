@@ -14,8 +14,8 @@
 //   l[row]      += 1 . P      v_mfma_f32_16x16x32
 // K in 16 bits (converted like V, four 16-bit products to the three) took 507 us where this takes 459: 16 sequences, 128 - 512
 // new tokens over 1 024 - 8 192 cached, 32 / 8 heads of 128; its LDS traffic is 4 / 5 of the other's 160 KB a step. With the
-// steps that all rows see freed of decisions, and the longest blocks first, it takes 362 us, 1.06 PFLOP/s: the matrix units are
-// busy 42 % of the clocks, the vector units (half of it exponentials, at a quarter of the rate) as long again, and the two
+// steps that all rows see freed of decisions, and the longest blocks first, it takes 359 us, 1.07 PFLOP/s: the matrix units are
+// busy 44 % of the clocks, the vector units (half of it exponentials, at a quarter of the rate) as long again, and the two
 // wavefronts of a SIMD overlap them little.
 // A value that is not finite has scale 255: it goes into LDS as zero, its token is noted, and the outputs of the rows that
 // see that token become NaN in the columns of its group; rows that do not see it are not touched by it.
