@@ -37,11 +37,9 @@
 
 namespace op::paged_attention_fp4::amd {
 
-using op::paged_attention::amd::BFloat16;
 using op::paged_attention::amd::clampPage;
 using op::paged_attention::amd::f32x4;
 using op::paged_attention::amd::fastExp2;
-using op::paged_attention::amd::Half;
 using op::paged_attention::amd::kHeadsPerWave;
 using op::paged_attention::amd::kLog2e;
 using op::paged_attention::amd::loadLane16ToLds;
@@ -172,26 +170,6 @@ struct Cut {
         return step < border ? step / (least + 1) : more + (step - border) / least;
     }
 };
-
-template <int BYTES> struct Bits;
-template <> struct Bits<2> { using type = uint16_t; };
-template <> struct Bits<4> { using type = uint32_t; };
-template <> struct Bits<8> { typedef unsigned type __attribute__((ext_vector_type(2))); };
-template <> struct Bits<16> { typedef unsigned type __attribute__((ext_vector_type(4))); };
-// ONCE: past the caches, for what a call reads once.
-template <int BYTES, bool ONCE = true>
-__device__ __forceinline__ void loadWords(const char *p, uint32_t *to) {
-    const auto *from = reinterpret_cast<const typename Bits<BYTES>::type *>(p);
-    const auto v = ONCE ? __builtin_nontemporal_load(from) : *from;
-    if constexpr (BYTES <= 4) {
-        to[0] = v;
-    } else {
-#pragma unroll
-        for (int i = 0; i < BYTES / 4; ++i) {
-            to[i] = v[i];
-        }
-    }
-}
 
 // How a head's elements and columns lie in the lanes. K: pieces of 128 (32 elements a lane) and, at 64 and 192, one of 64 (16
 // elements). V: one strip of HEAD / 16 neighbouring columns a lane, at head 192 a strip of 8 columns out of the first 128 and

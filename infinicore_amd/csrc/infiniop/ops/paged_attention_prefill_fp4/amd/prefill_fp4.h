@@ -38,12 +38,24 @@ using op::paged_attention::amd::waveInclusiveSum;
 using op::paged_attention::amd::waveMaxInt;
 using op::paged_attention_fp4::amd::IndexType;
 using op::paged_attention_fp4::amd::loadIndexOf;
-using op::paged_attention_fp4::amd::loadWords;
 using op::paged_attention_fp4::amd::PoolSide;
 namespace mx = device::amd::mx;
 
 constexpr int kTile = 16;          // tokens of a matrix instruction
 constexpr float kLazyLog2 = 8.0f;  // how far (in powers of two) a row maximum may outgrow its reference point
+
+// Two or four dwords of codes, through the caches: several row blocks read them.
+template <int WORDS>
+__device__ __forceinline__ void loadWords(const char *from, uint32_t *to) {
+    static_assert(WORDS == 2 || WORDS == 4, "8 or 16 bytes");
+    if constexpr (WORDS == 2) {
+        const uint2 x = *reinterpret_cast<const uint2 *>(from);
+        to[0] = x.x, to[1] = x.y;
+    } else {
+        const uint4 x = *reinterpret_cast<const uint4 *>(from);
+        to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+    }
+}
 
 struct PrefillFp4Args {
     void *out;
@@ -375,7 +387,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args
 #pragma unroll
             for (int p = 0; p < kPassesK; ++p) {
                 if (hasK(p)) {
-                    loadWords<16, false>(k_codes + kRow(p) * a.k_codes.row + 16 * kChunkOf(p), raw.k[p]);
+                    loadWords<4>(k_codes + kRow(p) * a.k_codes.row + 16 * kChunkOf(p), raw.k[p]);
                     raw.ks[p] = static_cast<uint8_t>(k_scales[kRow(p) * a.k_scales.row + kChunkOf(p)]);
                 }
             }
@@ -383,7 +395,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args
 #pragma unroll
             for (int p = 0; p < kPasses; ++p) {
                 if (hasV(p)) {
-                    loadWords<4 * G::kUnitWords, false>(v_codes + vRow(p) * a.v_codes.row + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
+                    loadWords<G::kUnitWords>(v_codes + vRow(p) * a.v_codes.row + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
                     raw.vs[p] = static_cast<uint8_t>(v_scales[vRow(p) * a.v_scales.row + vUnitOf(p) * G::kUnit / 32]);
                 }
             }
@@ -393,14 +405,14 @@ __global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args
             for (int p = 0; p < kPassesK; ++p) {
                 const int id = __shfl(ids, kRow(p) & 15, 64), row = __shfl(row_in_page, kRow(p) & 15, 64);
                 if (hasK(p)) {
-                    loadWords<16, false>(rowOf(a.k_codes, id, row) + 16 * kChunkOf(p), raw.k[p]);
+                    loadWords<4>(rowOf(a.k_codes, id, row) + 16 * kChunkOf(p), raw.k[p]);
                     raw.ks[p] = static_cast<uint8_t>(rowOf(a.k_scales, id, row)[kChunkOf(p)]);
                 }
             }
 #pragma unroll
             for (int p = 0; p < kPasses; ++p) {
                 if (hasV(p)) { // (vRow is the lane's own token)
-                    loadWords<4 * G::kUnitWords, false>(rowOf(a.v_codes, ids, row_in_page) + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
+                    loadWords<G::kUnitWords>(rowOf(a.v_codes, ids, row_in_page) + vUnitOf(p) * (G::kUnit / 2), raw.v[p]);
                     raw.vs[p] = static_cast<uint8_t>(rowOf(a.v_scales, ids, row_in_page)[vUnitOf(p) * G::kUnit / 32]);
                 }
             }
