@@ -209,9 +209,9 @@ template <int BM>
 constexpr int kTailSteps = BM / 64 + 1;
 
 // WHOLE: the page size is a multiple of 16, so that a tile lies in one page; otherwise every lane looks its rows up.
-// WAVES: 4, or 8 where a tile takes two passes of 64 lanes. Two wavefronts share a SIMD.
+// WAVES: 4, or 8 where a tile takes two passes of 64 lanes. Two wavefronts share a SIMD, but for four at head 256 (LDS).
 template <typename T, int HEAD, int R, int WAVES, bool WHOLE>
-__global__ void __launch_bounds__(64 * WAVES, 2) prefillFp4Kernel(PrefillFp4Args a) {
+__global__ void __launch_bounds__(64 * WAVES, HEAD == 256 && WAVES == 4 ? 1 : 2) prefillFp4Kernel(PrefillFp4Args a) {
     using S = typename T::storage;
     using G = Rows<HEAD>;
     constexpr int BM = 16 * R * WAVES, BN = kStep, TT = kTiles;
